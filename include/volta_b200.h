@@ -80,8 +80,14 @@ typedef enum vb_ns_mode {
      * (<= 1e-5) at tensor-core speed, but not bit-identical to the CPU arithmetic.  Updates far
      * smaller than sqrt(1e-8), whose normalised form is tiny (src/nn/optim/muon.rs:59), are held
      * with a larger power of two so that the bound covers them as well. */
-    VB_NS_F32_TC = 2
+    VB_NS_F32_TC = 2,
+    /* Newton-Schulz plans only (vb_ns_plan_create): f16 operands on the tensor cores, f32
+     * accumulation; the rate of VB_NS_BF16 with three more significand bits. */
+    VB_NS_F16 = 3
 } vb_ns_mode;
+
+/* Element types of caller-owned matrices. */
+typedef enum vb_dtype { VB_DTYPE_F32 = 0, VB_DTYPE_BF16 = 1, VB_DTYPE_F16 = 2 } vb_dtype;
 
 /* Flags of vb_optimizer_step_ex. */
 #define VB_STEP_DEFAULT 0u
@@ -502,6 +508,92 @@ int vb_multi_tensor_step_static(vb_engine *engine, const vb_optimizer_step_param
                                 int64_t n_tensors, const int64_t *sizes, void *const *params,
                                 const void *const *grads, void *const *state1,
                                 void *const *state2);
+
+/* ---- Newton-Schulz on caller-owned device matrices --------------------------------- */
+
+/* A plan holds what a list of matrix shapes needs to be orthogonalised together: the schedule of
+ * products, the workspace (vb_ns_plan_workspace) and the coefficients.  Both operators below run
+ * on it; their counterpart in the reference is the loop over parameters in Muon::step
+ * (src/nn/optim/muon.rs:108-163) with newton_schulz (muon.rs:50-103), here for the caller's
+ * buffers, types and strides, as vb_multi_tensor_step is for Adam and SGD.
+ *
+ * For every matrix U (rows x cols, the short side n, the long side m):
+ *     X_0 = U / (|U|_F + eps)
+ *     X_{k+1} = a_k X_k + b_k (X_k X_k^T) X_k + c_k (X_k X_k^T)^2 X_k         k = 0 .. n_steps - 1
+ *     O = X_{n_steps}
+ * with X^T X on the other side where rows > cols.  coefficients is {a_0, b_0, c_0, a_1, ...};
+ * muon.rs:67-100 is {1.5, -0.5, 0} in every step.  The coefficients must be finite and keep the
+ * singular values of every iterate below 2^20 for inputs in [0, 1], else VB_ERR_INVALID_ARG.
+ *
+ * ns_mode: VB_NS_F16 holds every iterate in f16 (times a power of two; the error of O is about
+ * 1e-3 relative on gradients with a floor of noise; singular directions that the input holds
+ * below about 2^-11 / sqrt(n) of the largest are lost, as in any 16-bit arithmetic), VB_NS_F32_TC in two f16
+ * planes (about 1e-6).  The other modes return VB_ERR_UNSUPPORTED.
+ *
+ * A matrix may have a side of 1 or 0; sides up to 65536.  A U of zeros gives zeros (eps > 0); a U
+ * with an infinity or a NaN gives NaN for that matrix and leaves the others as they are.  Results do not depend on
+ * what else the plan holds beyond the choice of a tile shape, and are the same bits in every call.
+ *
+ * All calls of one plan use its workspace: they are ordered by the engine's stream and must not
+ * overlap otherwise (two graphs captured from one plan must not run at the same time).  The calls
+ * allocate nothing, do not wait, and can be captured from the engine's stream into a graph, which then
+ * holds the buffers' addresses and the scalars of the call. */
+typedef struct vb_ns_plan vb_ns_plan;
+typedef struct vb_ns_matrices vb_ns_matrices;
+
+/* Pure host planning, no CUDA call: the products that a plan runs for one matrix (VB_NS_F16 and
+ * VB_NS_F32_TC alike), for hosts and tests that want to check or cost the schedule.  Buffers 0
+ * and 1 hold the working matrix X (n x m), 2 .. 6 short-side matrices; product k computes
+ *     D = e E + f F + g A B'      (B' = B for an update of X, else B^T), times s^scale_power
+ * where X_0 = s * (buffer 0).  ints: 9 per product {stage, A, B, E, F, D, scale_power, update, gram},
+ * -1 for an absent term; products of one stage are independent.  doubles: 3 per product {e, f, g}.
+ * The result is the last product's D times *final_scale.  Arrays may be NULL to query *n_products. */
+int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *coefficients, int64_t capacity,
+                          int64_t *n_products, int32_t *ints, double *doubles, double *final_scale);
+
+int vb_ns_plan_create(vb_engine *engine, int64_t n_matrices, const int64_t *rows, const int64_t *cols, int n_steps,
+                      const float *coefficients, float eps, int ns_mode, vb_ns_plan **out);
+/* Waits for the engine's stream, then frees the workspace.  Lists of the plan must not be used after it. */
+int vb_ns_plan_destroy(vb_ns_plan *plan);
+int vb_ns_plan_workspace(vb_ns_plan *plan, size_t *bytes);
+/* FLOPs of the products that one call launches (two per multiply-add; whole tiles, symmetric
+ * products counted by the tiles that are computed). */
+int vb_ns_plan_flops(vb_ns_plan *plan, double *flops);
+
+/* One array per matrix of the plan, in the caller's memory: pointers[i] is a device address of
+ * the engine's device, element (r, c) lies at pointers[i][r * strides[2 i] + c * strides[2 i + 1]]
+ * (in elements, >= 0; strides NULL: contiguous rows).  Pointers must be aligned to the element
+ * size; rows or columns on 16-byte boundaries are read fastest.  pointers[i] may be NULL for
+ * matrices without elements, and for an absent gradient.  The list keeps the addresses, not the memory, which
+ * must stay allocated while the list is used.  It is checked here, once. */
+int vb_ns_matrices_create(vb_ns_plan *plan, int dtype, void *const *pointers, const int64_t *strides,
+                          vb_ns_matrices **out);
+int vb_ns_matrices_destroy(vb_ns_matrices *list);
+
+/* outputs[i] = O(inputs[i]) for every matrix.  A list whose arrays are written must not hold two
+ * elements at one address; an output may be its own input (the same list).  Other overlaps are
+ * the caller's to avoid. */
+int vb_orthogonalize(vb_ns_plan *plan, const vb_ns_matrices *inputs, const vb_ns_matrices *outputs);
+
+/* Muon's step on the caller's buffers:
+ *     v <- momentum v + g;   u = nesterov ? g + momentum v : v;
+ *     p <- p (1 - lr weight_decay) - lr scales[i] O(u)
+ * in f32, each result rounded once to its array's type (u is not rounded to the velocity's).
+ * scales: one factor per matrix (NULL: 1).  muon.rs:133-160 is weight_decay 0 and scales 0.1.
+ * Matrices whose gradient is NULL are skipped with their velocity (muon.rs:110). */
+typedef struct vb_muon_step_params {
+    float lr;
+    float momentum;
+    float weight_decay;
+    int32_t nesterov;
+} vb_muon_step_params;
+int vb_muon_multi_tensor_step(vb_ns_plan *plan, const vb_muon_step_params *hp, const vb_ns_matrices *params,
+                              const vb_ns_matrices *grads, const vb_ns_matrices *velocities, const float *scales);
+
+/* Test hook, as vb_debug_muon_withhold_loads: the first product launch of the plan's next call withholds its loads
+ * with `wait_limit` polls per wait (0 = default).  The call returns VB_OK and stores neither outputs nor
+ * parameters; the next call that waits for the stream, and every later call on the plan, returns VB_ERR_TIMEOUT. */
+int vb_debug_ns_plan_withhold_loads(vb_ns_plan *plan, uint32_t wait_limit);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,7 @@ STATUS_NAMES = {
 VB_NS_F32 = 0
 VB_NS_BF16 = 1
 VB_NS_F32_TC = 2
+VB_NS_F16 = 3
 VB_STEP_DEFAULT = 0
 VB_STEP_NO_EXCHANGE = 1
 VB_STEP_EXCHANGE_BF16 = 2
@@ -41,6 +42,12 @@ class StepParams(C.Structure):
     _fields_ = [("op", C.c_uint32), ("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float),
                 ("t", C.c_float), ("eps", C.c_float), ("weight_decay", C.c_float),
                 ("padding", C.c_float)]
+
+
+class MuonStepParams(C.Structure):
+    """Mirror of ``vb_muon_step_params``."""
+
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("nesterov", C.c_int32)]
 
 
 _vp = C.c_void_p
@@ -130,6 +137,17 @@ SIGNATURES = {
     "vb_muon_last_ns_flops": [_vp, C.POINTER(C.c_double)],
     "vb_multi_tensor_step": [_vp, C.POINTER(StepParams), _i64, _i64p, _vpp, _vpp, _vpp, _vpp],
     "vb_multi_tensor_step_static": [_vp, C.POINTER(StepParams), _i64, _i64p, _vpp, _vpp, _vpp, _vpp],
+    "vb_plan_newton_schulz": [_i64, _i64, C.c_int, _f32p, _i64, _i64p, C.POINTER(C.c_int32), C.POINTER(C.c_double),
+                              C.POINTER(C.c_double)],
+    "vb_ns_plan_create": [_vp, _i64, _i64p, _i64p, C.c_int, _f32p, C.c_float, C.c_int, _vpp],
+    "vb_ns_plan_destroy": [_vp],
+    "vb_ns_plan_workspace": [_vp, C.POINTER(C.c_size_t)],
+    "vb_ns_plan_flops": [_vp, C.POINTER(C.c_double)],
+    "vb_ns_matrices_create": [_vp, C.c_int, _vpp, _i64p, _vpp],
+    "vb_ns_matrices_destroy": [_vp],
+    "vb_orthogonalize": [_vp, _vp, _vp],
+    "vb_muon_multi_tensor_step": [_vp, C.POINTER(MuonStepParams), _vp, _vp, _vp, _f32p],
+    "vb_debug_ns_plan_withhold_loads": [_vp, C.c_uint32],
 }
 OTHER_SYMBOLS = ["vb_abi_version", "vb_last_error"]
 

@@ -683,6 +683,7 @@ int vb_engine_destroy(vb_engine *e)
     if (!e) return VB_OK;
     cudaSetDevice(e->device);
     if (e->stream) cudaStreamSynchronize(e->stream);
+    for (vb_ns_plan *plan : e->ns_plans) ns_plan_orphan(plan);
     comm_destroy(e);
     for (int ph = 0; ph < VB_PHASE_COUNT; ++ph) {
         for (auto &pr : e->prof_pairs[ph]) {
@@ -719,6 +720,7 @@ static int engine_device_errors(vb_engine *e)
         VB_TRY(fence_check_error(opt));
         if (opt->kind == KIND_MUON) VB_TRY(muon_check_error(opt));
     }
+    for (vb_ns_plan *plan : e->ns_plans) VB_TRY(ns_plan_check_error(plan));
     return VB_OK;
 }
 

@@ -40,6 +40,7 @@ struct vb_engine {
     uint64_t checked_sets[4] = {0, 0, 0, 0};
     int checked_next = 0;
     std::vector<vb_optimizer *> optimizers;  // alive optimizers of this engine (their error words are read on synchronize)
+    std::vector<vb_ns_plan *> ns_plans;      // alive Newton-Schulz plans, for the same reason
     cudaEvent_t deadline_event = nullptr;  // vb_engine_synchronize_deadline
     uint32_t wait_limit_ms = 5000;         // bound of every device-side wait on another rank
     double replicated_fraction = 0.0;      // Adam/SGD optimizers created from now on: share of the arena every rank updates itself
@@ -128,6 +129,10 @@ float *muon_velocity_ptr(vb_optimizer *opt, int64_t tensor);  // nullptr if not 
 void plan_muon_owners(int64_t n, const int64_t *rows, const int64_t *cols, int world, int ns_mode, int ns_steps,
                       int *owner_out);
 double muon_tensor_cost(int64_t rows, int64_t cols, int ns_mode, int ns_steps);  // estimated seconds per step
+
+// ns_plan.cu
+int ns_plan_check_error(vb_ns_plan *plan);  // VB_ERR_TIMEOUT once a product kernel of the plan gave up a wait
+void ns_plan_orphan(vb_ns_plan *plan);      // the engine goes away before the plan
 
 // comm.cpp
 int comm_unique_id(void *id128);

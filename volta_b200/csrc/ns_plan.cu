@@ -1,0 +1,754 @@
+// Newton-Schulz on caller-owned matrices: the planner, the workspace and the C entry points
+// (include/volta_b200.h, vb_ns_plan_*, vb_orthogonalize, vb_muon_multi_tensor_step).
+//
+// The iteration X' = q(G) X with G = X X^T and q(t) = a + b t + c t^2 is run in groups of steps.
+// Inside a group everything is a polynomial of the group's first Gram, so it stays on the short side:
+//     G      = X X^T                                    n^2 m   (symmetric: half a product)
+//     R      = b G + c G G                              n^3     (q(G) = a I + R)
+//     T      = a G + R G;     P' = a P + alpha R + R P   n^3 each (alpha I + P: the group's polynomial so far)
+//     G'     = a T + T R                                n^3     (the Gram of the next iterate: q(G)^2 G)
+//     X'     = alpha X + P X                            2 n^2 m (once per group)
+// The longer a group, the less is paid on the long side: a step by itself costs 3 n^2 m + n^3, every
+// further one of a group 4 n^3.  What limits a group is rounding: noise of size d in G (2^-12 |G|_F
+// spread over the spectrum) grows by the slope of t q(t)^2 with every step and reaches small eigenvalues'
+// q after k steps as d prod a^2.  In f16 the 1024-sided quintic run as one group is wrong by 10 to
+// 100 % on gradients with a decaying spectrum.  The first group of a call may amplify 150-fold (its Gram has
+// trace 1, so d is small), later ones, whose Gram is near the identity, 17-fold: with these limits
+// the error equals that of one step at a time (1e-3 to 4e-3 relative) on Gaussian, low-rank-plus-noise
+// and power-law spectra.  For the usual quintic this means groups of 3 and 2.  Matrices whose long
+// side is less than 1.5 times the short one run one step at a time: grouping saves nothing there.
+//
+// Powers of two.  Every stored matrix carries 2^e with e from the largest value its polynomial takes
+// on [0, 1] (sampled), so that f16 neither overflows nor loses small entries.
+#include <cmath>
+
+#include <algorithm>
+#include <memory>
+#include <numeric>
+
+#include "engine.h"
+#include "ns_plan.h"
+
+namespace vb {
+namespace {
+
+constexpr int kSquares = 5;  // short-side matrices alive at once: G, T, R, P and the one being written
+constexpr int kMaxSteps = 64;
+constexpr int64_t kMaxSide = 65536;
+constexpr double kFirstGroupGain = 150.0, kGroupGain = 17.0;
+constexpr double kDiverged = 1048576.0;
+// norm and gather of a batch follow each other; a batch's arrays should stay in the 126 MB L2 in between
+constexpr int64_t kBatchElements = 8 << 20;
+
+// ---- schedule ----------------------------------------------------------------------------
+enum BufferId { BUF_X0 = 0, BUF_X1 = 1, BUF_SQUARE = 2 };  // BUF_SQUARE + k: k-th short-side matrix
+
+struct Product {
+    int A, B, E, F, D;  // buffers; E, F may be -1
+    double e, f, g;
+    int scale_power;
+    bool update;     // M x N x K = n x m x n with B = X; otherwise n x n, symmetric
+    bool gram;       // K = m
+};
+struct Schedule {
+    std::vector<std::vector<Product>> stages;  // products of a stage are independent
+    int final_buffer = BUF_X0;
+    double final_scale = 1.0;  // 2^-e of the last iterate
+};
+
+struct Step {
+    double a, b, c;
+    double q(double t) const { return a + t * (b + c * t); }
+};
+
+int exponent_for(double bound)
+{
+    // twice the bound below 2^15: rounding noise may push eigenvalues past the polynomial's range
+    const int e = (int)std::floor(14.0 - std::log2(std::max(bound, 1e-12)));
+    return std::min(e, 40);
+}
+
+std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, bool grouped)
+{
+    std::vector<std::vector<int>> groups;
+    std::vector<double> lam(4097);
+    for (size_t i = 0; i < lam.size(); ++i) lam[i] = (double)i / (double)(lam.size() - 1);
+    double gain = 1.0;
+    for (int k = 0; k < (int)steps.size(); ++k) {
+        const Step &s = steps[(size_t)k];
+        const bool fits = grouped && !groups.empty() && gain <= (groups.size() == 1 ? kFirstGroupGain : kGroupGain);
+        if (!fits) {
+            groups.emplace_back();
+            gain = 1.0;
+        }
+        groups.back().push_back(k);
+        // steepest slope of t q(t)^2 on the range the eigenvalues are in
+        double top = 0.0, slope = s.a * s.a;
+        for (double t : lam) top = std::max(top, t);
+        for (int i = 0; i <= 1024; ++i) {
+            const double t = top * i / 1024.0, q = s.q(t);
+            slope = std::max(slope, std::fabs(q * q + 2.0 * t * q * (s.b + 2.0 * s.c * t)));
+        }
+        gain *= slope;
+        for (double &t : lam) t = t * s.q(t) * s.q(t);
+    }
+    return groups;
+}
+
+// Returns false if the iterates leave the range that is sensible to hold.
+bool make_schedule(const std::vector<Step> &steps, bool grouped, Schedule *out)
+{
+    const auto groups = make_groups(steps, grouped);
+    const int kSamples = 8192;
+    std::vector<double> lam, sv;  // samples of the spectrum: of G, and the singular values of X
+    for (int i = 0; i <= kSamples; ++i) lam.push_back((double)i / kSamples);
+    for (int i = 0; i < 256; ++i) lam.push_back(std::exp2(-i / 8.0));
+    for (double t : lam) sv.push_back(std::sqrt(t));
+    auto bound = [&](auto &&fn) {
+        double top = 0.0;
+        for (size_t i = 0; i < lam.size(); ++i) top = std::max(top, std::fabs(fn(i)));
+        return top;
+    };
+    int x = BUF_X0, ex = 0;  // the first working matrix has a scale of its own (on the device)
+    for (size_t gi = 0; gi < groups.size(); ++gi) {
+        const bool first = gi == 0;
+        auto square = [&](std::initializer_list<int> live) {
+            for (int k = BUF_SQUARE; k < BUF_SQUARE + kSquares; ++k)
+                if (std::find(live.begin(), live.end(), k) == live.end()) return k;
+            return -1;
+        };
+        int G = BUF_SQUARE, P = -1, eP = 0;
+        int eG = exponent_for(bound([&](size_t i) { return lam[i]; }));
+        out->stages.push_back({{x, x, -1, -1, G, 0.0, 0.0, std::exp2(eG - 2 * ex), first ? 2 : 0, false, true}});
+        double alpha = 1.0, fP = 1.0;  // the group's polynomial is alpha I + fP P
+        std::vector<double> poly(lam.size(), 1.0);
+        for (size_t k = 0; k < groups[gi].size(); ++k) {
+            const Step s = steps[(size_t)groups[gi][k]];
+            const bool last = k + 1 == groups[gi].size();
+            // R, held as fR times a stored matrix: a linear step's R is b G itself
+            int R = G, eR = eG;
+            double fR = s.b;
+            if (s.c != 0.0) {
+                R = square({G, P});
+                eR = exponent_for(bound([&](size_t i) { return lam[i] * (s.b + s.c * lam[i]); }));
+                fR = 1.0;
+                out->stages.push_back({{G, G, G, -1, R, s.b * std::exp2(eR - eG), 0.0, s.c * std::exp2(eR - 2 * eG), 0, false, false}});
+            }
+            std::vector<Product> both;
+            int T = -1, eT = 0;
+            if (!last) {
+                T = square({G, R, P});
+                eT = exponent_for(bound([&](size_t i) { return lam[i] * s.q(lam[i]); }));
+                both.push_back({R, G, G, -1, T, s.a * std::exp2(eT - eG), 0.0, fR * std::exp2(eT - eR - eG), 0, false, false});
+            }
+            for (size_t i = 0; i < lam.size(); ++i) poly[i] *= s.q(lam[i]);
+            if (P < 0) {
+                P = R, eP = eR, fP = fR;
+            } else {
+                const double next = alpha * s.a;
+                const int N = square({G, R, P, T});
+                const int eN = exponent_for(bound([&](size_t i) { return poly[i] - next; }));
+                both.push_back({R, P, P, R, N, s.a * fP * std::exp2(eN - eP), alpha * fR * std::exp2(eN - eR),
+                                fR * fP * std::exp2(eN - eR - eP), 0, false, false});
+                P = N, eP = eN, fP = 1.0;
+            }
+            alpha *= s.a;
+            if (!both.empty()) out->stages.push_back(both);
+            for (double &t : lam) t = t * s.q(t) * s.q(t);
+            if (!last) {
+                const int N = square({T, R, P});
+                const int eN = exponent_for(bound([&](size_t i) { return lam[i]; }));
+                out->stages.push_back({{T, R, T, -1, N, s.a * std::exp2(eN - eT), 0.0, fR * std::exp2(eN - eT - eR), 0, false, false}});
+                G = N, eG = eN;
+            }
+        }
+        for (size_t i = 0; i < sv.size(); ++i) sv[i] *= poly[i];
+        const double top = bound([&](size_t i) { return sv[i]; });
+        if (!(top < kDiverged)) return false;
+        const int eX = exponent_for(top), y = x == BUF_X0 ? BUF_X1 : BUF_X0;
+        out->stages.push_back({{P, x, x, -1, y, alpha * std::exp2(eX - ex), 0.0, fP * std::exp2(eX - eP - ex), first ? 1 : 0, true, false}});
+        x = y, ex = eX;
+    }
+    out->final_buffer = x;
+    out->final_scale = std::exp2(-ex);
+    return true;
+}
+
+const char *const kDivergedText = "these coefficients take singular values in [0, 1] beyond 2^20";
+
+int read_steps(int n_steps, const float *coefficients, std::vector<Step> *steps)
+{
+    if (n_steps < 1 || n_steps > kMaxSteps || !coefficients)
+        return fail(VB_ERR_INVALID_ARG, "1 to %d steps with coefficients are needed", kMaxSteps);
+    for (int k = 0; k < n_steps; ++k) {
+        const Step s{coefficients[3 * k], coefficients[3 * k + 1], coefficients[3 * k + 2]};
+        if (!std::isfinite(s.a) || !std::isfinite(s.b) || !std::isfinite(s.c))
+            return fail(VB_ERR_INVALID_ARG, "coefficients of step %d are not finite", k);
+        steps->push_back(s);
+    }
+    return VB_OK;
+}
+bool runs_grouped(int64_t rows, int64_t cols) { return 2 * std::max(rows, cols) >= 3 * std::min(rows, cols); }
+
+struct Launch {
+    NsLaunch l;
+    int shape;
+};
+
+struct DeviceGuard {  // runs the call on the engine's device and leaves the caller's current one as it was
+    int before = -1;
+    int enter(int device)
+    {
+        VB_CUDA(cudaGetDevice(&before));
+        if (before == device) before = -1;
+        else VB_CUDA(cudaSetDevice(device));
+        return VB_OK;
+    }
+    ~DeviceGuard()
+    {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+}  // namespace
+}  // namespace vb
+
+struct vb_ns_matrices {
+    vb_ns_plan *plan = nullptr;
+    int dtype = 0;
+    std::vector<vb::NsArray> arrays;  // in the working orientation
+    std::vector<uint8_t> vec;         // rows (or columns) on 16-byte boundaries
+    bool writable = true;             // no two elements at one address
+    bool any_null = false;            // a matrix with elements has no array
+    const char *why = "";             // why it is not writable
+};
+
+struct vb_ns_plan {
+    vb_engine *eng = nullptr;
+    int device = 0;
+    int64_t n = 0;
+    std::vector<int64_t> rows, cols;
+    std::vector<vb::NsMatrixDims> dims;
+    int planes = 1;
+    float eps = 0.0f;
+    double flops = 0.0;
+    size_t workspace = 0;
+    char *d_base = nullptr;  // one allocation: everything below lies in it
+    vb::NsElementwise ew{};  // device pointers of the element-wise passes
+    const int32_t *d_tile_matrix = nullptr;
+    std::vector<vb::Launch> launches;
+    struct Batch {
+        int32_t first, count, tile0, n_tiles;
+    };
+    std::vector<Batch> batches;
+    vb::NsError error{};
+    uint32_t *h_error = nullptr;
+    bool withhold = false;
+    uint32_t wait_limit = 0;
+    std::unique_ptr<vb::NsBatchArgs> args;  // scratch of a call
+};
+
+namespace vb {
+
+int ns_plan_check_error(vb_ns_plan *p)
+{
+    if (p->h_error && *reinterpret_cast<volatile uint32_t *>(p->h_error) != 0)
+        return fail(VB_ERR_TIMEOUT, "a Newton-Schulz product kernel gave up waiting on a pipeline barrier (role %u)", *p->h_error);
+    return VB_OK;
+}
+void ns_plan_orphan(vb_ns_plan *p) { p->eng = nullptr; }
+
+namespace {
+
+void free_plan(vb_ns_plan *p)
+{
+    if (p->d_base) cudaFree(p->d_base);
+    if (p->h_error) cudaFreeHost(p->h_error);
+    delete p;
+}
+
+// Device addresses of the parts of the workspace, in the order they are asked for.
+struct Carver {
+    char *base = nullptr;
+    size_t used = 0;
+    template <typename T>
+    T *take(size_t count)
+    {
+        used = (used + 1023) / 1024 * 1024;
+        T *p = reinterpret_cast<T *>(base + used);
+        used += count * sizeof(T);
+        return p;
+    }
+};
+
+int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
+{
+    Schedule schedules[2];
+    for (int g = 0; g < 2; ++g)
+        if (!make_schedule(steps, g == 1, &schedules[g]))
+            return fail(VB_ERR_INVALID_ARG, kDivergedText);
+    const int64_t n = p->n;
+    std::vector<int> kind((size_t)n);
+    std::vector<int32_t> tile_matrix;
+    std::vector<int64_t> square_off((size_t)n);
+    int64_t x_total = 0, square_total = 0, tiles = 0, batch_elements = 0;
+    p->dims.resize((size_t)n);
+    for (int64_t i = 0; i < n; ++i) {
+        NsMatrixDims &d = p->dims[(size_t)i];
+        d = NsMatrixDims{};
+        d.n = (int32_t)std::min(p->rows[i], p->cols[i]);
+        d.m = (int32_t)std::max(p->rows[i], p->cols[i]);
+        if (d.n == 0) d.m = 0;
+        d.np = (int32_t)round_up(d.n, kNsPad);
+        d.mp = (int32_t)round_up(d.m, kNsPad);
+        kind[(size_t)i] = runs_grouped(d.n, d.m) ? 1 : 0;
+        const Schedule &s = schedules[kind[(size_t)i]];
+        d.x_off = x_total;
+        d.final_off = s.final_buffer;  // buffer number for now
+        d.final_scale = (float)s.final_scale;
+        square_off[(size_t)i] = square_total;
+        x_total += (int64_t)p->planes * d.np * d.mp;
+        square_total += (int64_t)kSquares * p->planes * d.np * d.np;
+        d.tile0 = (int32_t)tiles;
+        d.n_tiles = (d.np / kNsTileI) * (d.mp / kNsTileJ);
+        tiles += d.n_tiles;
+        if (tiles > INT32_MAX) return fail(VB_ERR_UNSUPPORTED, "the plan's matrices have too many elements");
+        tile_matrix.insert(tile_matrix.end(), (size_t)d.n_tiles, (int32_t)i);
+        const int64_t elements = (int64_t)d.n * d.m;
+        if (p->batches.empty() || p->batches.back().count == kNsBatch || batch_elements + elements > kBatchElements) {
+            p->batches.push_back({(int32_t)i, 0, d.tile0, 0});
+            batch_elements = 0;
+        }
+        batch_elements += elements;
+        p->batches.back().count += 1;
+        p->batches.back().n_tiles += d.n_tiles;
+    }
+    for (auto &d : p->dims) d.final_off = d.x_off + (d.final_off == BUF_X1 ? x_total : 0);
+
+    // stages of all matrices side by side: launch k runs every matrix's k-th stage
+    struct HostLaunch {
+        std::vector<NsProduct> problems;
+        std::vector<NsTile> tiles;
+        int shape;
+    };
+    std::vector<HostLaunch> launches;
+    size_t n_launches = 0;
+    for (int64_t i = 0; i < n; ++i)
+        if (p->dims[(size_t)i].n > 0) n_launches = std::max(n_launches, schedules[kind[(size_t)i]].stages.size());
+    launches.resize(n_launches);
+
+    // The carving is done twice: for the size, then with the addresses (tensor maps need them).
+    __half *x_base = nullptr, *square_base = nullptr;
+    for (int round = 0; round < 2; ++round) {
+        Carver c;
+        c.base = p->d_base;
+        x_base = c.take<__half>((size_t)(2 * x_total));
+        square_base = c.take<__half>((size_t)square_total);
+        p->ew.x = x_base;
+        p->ew.partials = c.take<double>((size_t)tiles);
+        p->ew.scale = c.take<float>((size_t)n);
+        p->ew.active = c.take<uint32_t>((size_t)n);
+        p->error.device = c.take<uint32_t>(1);
+        p->ew.error = p->error.device;
+        NsMatrixDims *d_dims = c.take<NsMatrixDims>((size_t)n);
+        int32_t *d_tile_matrix = c.take<int32_t>(tile_matrix.size());
+        p->ew.dims = d_dims;
+        p->d_tile_matrix = d_tile_matrix;
+        for (size_t k = 0; k < n_launches; ++k) {
+            HostLaunch &hl = launches[k];
+            hl.problems.clear();
+            hl.tiles.clear();
+            for (int64_t i = 0; i < n; ++i) {
+                const NsMatrixDims &d = p->dims[(size_t)i];
+                const Schedule &s = schedules[kind[(size_t)i]];
+                if (d.n == 0 || k >= s.stages.size()) continue;
+                const int64_t xp = (int64_t)d.np * d.mp, sp = (int64_t)d.np * d.np;
+                auto address = [&](int buffer) -> __half * {
+                    if (buffer < 0) return nullptr;
+                    if (buffer == BUF_X0) return x_base + d.x_off;
+                    if (buffer == BUF_X1) return x_base + x_total + d.x_off;
+                    return square_base + square_off[(size_t)i] + (int64_t)(buffer - BUF_SQUARE) * p->planes * sp;
+                };
+                for (const Product &pr : s.stages[k]) {
+                    NsProduct q{};
+                    q.M = d.np;
+                    q.N = pr.update ? d.mp : d.np;
+                    q.K = pr.gram ? d.mp : d.np;
+                    q.ld = q.N;
+                    q.plane_rows_a = q.plane_rows_b = d.np;
+                    q.plane_d = pr.update ? xp : sp;
+                    q.E = address(pr.E);
+                    q.F = address(pr.F);
+                    q.D = address(pr.D);
+                    q.e = (float)pr.e, q.f = (float)pr.f, q.g = (float)pr.g;
+                    q.scale_power = pr.scale_power;
+                    q.scale = p->ew.scale + i;
+                    q.matrix = (int32_t)i;
+                    q.flags = pr.update ? NS_B_MN_MAJOR : 0;
+                    if (round == 1) {
+                        VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, (int64_t)p->planes * d.np, false));
+                        VB_TRY(make_ns_map(&q.map_b, address(pr.B), pr.update ? q.N : q.K, (int64_t)p->planes * d.np, pr.update));
+                    }
+                    hl.problems.push_back(q);
+                }
+            }
+            // long contractions first: the tail of a launch is then made of short ones
+            std::stable_sort(hl.problems.begin(), hl.problems.end(), [](const NsProduct &a, const NsProduct &b) { return a.K > b.K; });
+            auto make_tiles = [&](int shape) {
+                int bm, bn;
+                ns_tile_extent(shape, &bm, &bn);
+                hl.tiles.clear();
+                hl.shape = shape;
+                for (size_t q = 0; q < hl.problems.size(); ++q) {
+                    const NsProduct &pr = hl.problems[q];
+                    const bool symmetric = (pr.flags & NS_B_MN_MAJOR) == 0;
+                    for (int m0 = 0; m0 < pr.M; m0 += bm)
+                        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn)
+                            hl.tiles.push_back({(int32_t)q, m0, n0, symmetric && n0 > m0 ? 1 : 0});
+                }
+            };
+            make_tiles(NS_TILE_PAIR_256);
+            if ((int)hl.tiles.size() < p->eng->sm_count / 2) make_tiles(NS_TILE_128);
+            NsProduct *d_problems = c.take<NsProduct>(hl.problems.size());
+            NsTile *d_tiles = c.take<NsTile>(hl.tiles.size());
+            if (round == 1) {
+                VB_CUDA(cudaMemcpyAsync(d_problems, hl.problems.data(), hl.problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
+                VB_CUDA(cudaMemcpyAsync(d_tiles, hl.tiles.data(), hl.tiles.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
+                p->launches.push_back({{d_problems, d_tiles, (int)hl.tiles.size()}, hl.shape});
+                int bm, bn;
+                ns_tile_extent(hl.shape, &bm, &bn);
+                for (const NsTile &t : hl.tiles)
+                    p->flops += 2.0 * (p->planes == 2 ? 3.0 : 1.0) * bm * bn * hl.problems[(size_t)t.problem].K;
+            }
+        }
+        if (round == 0) {
+            p->workspace = c.used;
+            VB_CUDA(cudaMalloc((void **)&p->d_base, std::max<size_t>(c.used, 1024)));
+        } else {
+            VB_CUDA(cudaMemsetAsync(p->error.device, 0, sizeof(uint32_t), p->eng->stream));
+            VB_CUDA(cudaMemcpyAsync(d_dims, p->dims.data(), (size_t)n * sizeof(NsMatrixDims), cudaMemcpyHostToDevice, p->eng->stream));
+            VB_CUDA(cudaMemcpyAsync(d_tile_matrix, tile_matrix.data(), tile_matrix.size() * sizeof(int32_t), cudaMemcpyHostToDevice, p->eng->stream));
+        }
+    }
+    VB_CUDA(cudaHostAlloc((void **)&p->h_error, sizeof(uint32_t), cudaHostAllocMapped));
+    *p->h_error = 0;
+    VB_CUDA(cudaHostGetDevicePointer((void **)&p->error.host, p->h_error, 0));
+    VB_CUDA(cudaStreamSynchronize(p->eng->stream));  // the host copies above go out of scope
+    return VB_OK;
+}
+
+// What both operators share: per batch `fill` sets the arrays of one matrix.
+template <typename Fill>
+int run_plan(vb_ns_plan *p, const NsElementwise &w, const NsElementwise &fin, bool step, Fill &&fill)
+{
+    vb_engine *e = p->eng;
+    NsBatchArgs &args = *p->args;
+    auto load = [&](const vb_ns_plan::Batch &b, bool finish) {
+        args.first = b.first;
+        args.count = b.count;
+        args.tile0 = b.tile0;
+        args.n_tiles = b.n_tiles;
+        for (int32_t k = 0; k < b.count; ++k) fill(b.first + k, args.m[k], finish);
+    };
+    for (const auto &b : p->batches) {
+        load(b, false);
+        VB_TRY(launch_ns_norm(w, args, p->d_tile_matrix, step, e->stream));
+        VB_TRY(launch_ns_gather(w, args, p->d_tile_matrix, step, e->stream));
+        if (b.n_tiles > 0) e->launches += 2;
+    }
+    for (const Launch &l : p->launches) {
+        VB_TRY(launch_ns_products(l.l, l.shape, p->planes, w.active, p->error, e->sm_count, e->stream, p->wait_limit, p->withhold));
+        p->withhold = false;
+        p->wait_limit = 0;
+        if (l.l.n_tiles > 0) e->launches += 1;
+    }
+    for (const auto &b : p->batches) {
+        load(b, true);
+        VB_TRY(launch_ns_finish(fin, args, p->d_tile_matrix, step, e->stream));
+        if (b.n_tiles > 0) e->launches += 1;
+    }
+    return VB_OK;
+}
+
+int check_list(const vb_ns_plan *p, const vb_ns_matrices *l, const char *name, bool written, bool may_be_absent)
+{
+    if (!l) return fail(VB_ERR_INVALID_ARG, "%s is null", name);
+    if (l->plan != p) return fail(VB_ERR_INVALID_ARG, "%s belongs to another plan", name);
+    if (l->any_null && !may_be_absent) return fail(VB_ERR_INVALID_ARG, "%s has a null pointer", name);
+    if (written && !l->writable) return fail(VB_ERR_INVALID_ARG, "%s cannot be written: %s", name, l->why);
+    return VB_OK;
+}
+// Two lists may share a matrix's memory only as the very same array.
+int check_alias(const vb_ns_matrices *a, const vb_ns_matrices *b, const char *names, bool same_allowed)
+{
+    for (size_t i = 0; i < a->arrays.size(); ++i) {
+        const NsArray &x = a->arrays[i], &y = b->arrays[i];
+        if (x.ptr == nullptr || x.ptr != y.ptr) continue;
+        if (!same_allowed || a->dtype != b->dtype || x.si != y.si || x.sj != y.sj)
+            return fail(VB_ERR_INVALID_ARG, "%s of matrix %lld start at one address", names, (long long)i);
+    }
+    return VB_OK;
+}
+
+int begin_call(vb_ns_plan *p, DeviceGuard *guard)
+{
+    if (!p) return fail(VB_ERR_INVALID_ARG, "plan is null");
+    if (!p->eng) return fail(VB_ERR_STATE, "the plan's engine has been destroyed");
+    VB_TRY(ns_plan_check_error(p));
+    return guard->enter(p->device);
+}
+
+}  // namespace
+}  // namespace vb
+
+using namespace vb;
+
+#define VB_NS_BEGIN try {
+#define VB_NS_END                                                                                    \
+    }                                                                                                \
+    catch (const std::bad_alloc &) { return fail(VB_ERR_STATE, "out of host memory"); }              \
+    catch (const std::exception &ex) { return fail(VB_ERR_STATE, "exception: %s", ex.what()); }      \
+    catch (...) { return fail(VB_ERR_STATE, "unknown exception"); }
+
+extern "C" {
+
+int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *coefficients, int64_t capacity,
+                          int64_t *n_products, int32_t *ints, double *doubles, double *final_scale)
+{
+    VB_NS_BEGIN
+    if (!n_products) return fail(VB_ERR_INVALID_ARG, "n_products is null");
+    if (rows < 0 || cols < 0) return fail(VB_ERR_INVALID_ARG, "negative side");
+    std::vector<Step> steps;
+    VB_TRY(read_steps(n_steps, coefficients, &steps));
+    Schedule s;
+    if (!make_schedule(steps, runs_grouped(rows, cols), &s)) return fail(VB_ERR_INVALID_ARG, kDivergedText);
+    int64_t k = 0;
+    for (size_t stage = 0; stage < s.stages.size(); ++stage)
+        for (const Product &p : s.stages[stage]) {
+            if (k < capacity && ints) {
+                const int32_t v[9] = {(int32_t)stage, p.A, p.B, p.E, p.F, p.D, p.scale_power, p.update, p.gram};
+                std::copy(v, v + 9, ints + 9 * k);
+            }
+            if (k < capacity && doubles) doubles[3 * k] = p.e, doubles[3 * k + 1] = p.f, doubles[3 * k + 2] = p.g;
+            ++k;
+        }
+    *n_products = k;
+    if (final_scale) *final_scale = s.final_scale;
+    if ((ints || doubles) && capacity < k) return fail(VB_ERR_INVALID_ARG, "%lld products, room for %lld", (long long)k, (long long)capacity);
+    return VB_OK;
+    VB_NS_END
+}
+
+int vb_ns_plan_create(vb_engine *e, int64_t n, const int64_t *rows, const int64_t *cols, int n_steps,
+                      const float *coefficients, float eps, int ns_mode, vb_ns_plan **out)
+{
+    VB_NS_BEGIN
+    if (!out) return fail(VB_ERR_INVALID_ARG, "out is null");
+    *out = nullptr;
+    if (!e) return fail(VB_ERR_INVALID_ARG, "engine is null");
+    if (n < 0 || n > (1 << 20) || (n > 0 && (!rows || !cols))) return fail(VB_ERR_INVALID_ARG, "bad list of %lld matrices", (long long)n);
+    std::vector<Step> steps;
+    VB_TRY(read_steps(n_steps, coefficients, &steps));
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(VB_ERR_INVALID_ARG, "eps must be finite and >= 0");
+    if (ns_mode != VB_NS_F16 && ns_mode != VB_NS_F32_TC)
+        return fail(ns_mode == VB_NS_F32 || ns_mode == VB_NS_BF16 ? VB_ERR_UNSUPPORTED : VB_ERR_INVALID_ARG,
+                    "a plan's ns_mode is VB_NS_F16 or VB_NS_F32_TC, not %d", ns_mode);
+    for (int64_t i = 0; i < n; ++i)
+        if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxSide || cols[i] > kMaxSide)
+            return fail(VB_ERR_INVALID_ARG, "matrix %lld is %lld x %lld: sides are 0 to %lld", (long long)i, (long long)rows[i], (long long)cols[i], (long long)kMaxSide);
+    DeviceGuard guard;
+    VB_TRY(guard.enter(e->device));
+    vb_ns_plan *p = new vb_ns_plan();
+    p->eng = e;
+    p->device = e->device;
+    p->n = n;
+    p->rows.assign(rows, rows + n);
+    p->cols.assign(cols, cols + n);
+    p->planes = ns_mode == VB_NS_F32_TC ? 2 : 1;
+    p->eps = eps;
+    int status;
+    try {
+        p->args.reset(new NsBatchArgs());
+        status = build_plan(p, steps);
+        if (status == VB_OK) e->ns_plans.push_back(p);
+    } catch (...) {
+        free_plan(p);
+        throw;
+    }
+    if (status != VB_OK) {
+        cudaStreamSynchronize(e->stream);
+        free_plan(p);
+        return status;
+    }
+    *out = p;
+    return VB_OK;
+    VB_NS_END
+}
+
+int vb_ns_plan_destroy(vb_ns_plan *p)
+{
+    if (!p) return VB_OK;
+    int before = -1;
+    cudaGetDevice(&before);
+    cudaSetDevice(p->device);
+    if (p->eng) {
+        cudaStreamSynchronize(p->eng->stream);
+        auto &all = p->eng->ns_plans;
+        all.erase(std::remove(all.begin(), all.end(), p), all.end());
+    }
+    free_plan(p);
+    if (before >= 0) cudaSetDevice(before);
+    return VB_OK;
+}
+
+int vb_ns_plan_workspace(vb_ns_plan *p, size_t *bytes)
+{
+    if (!p || !bytes) return fail(VB_ERR_INVALID_ARG, "null argument");
+    *bytes = p->workspace;
+    return VB_OK;
+}
+
+int vb_ns_plan_flops(vb_ns_plan *p, double *flops)
+{
+    if (!p || !flops) return fail(VB_ERR_INVALID_ARG, "null argument");
+    *flops = p->flops;
+    return VB_OK;
+}
+
+int vb_ns_matrices_create(vb_ns_plan *p, int dtype, void *const *pointers, const int64_t *strides, vb_ns_matrices **out)
+{
+    VB_NS_BEGIN
+    if (!out) return fail(VB_ERR_INVALID_ARG, "out is null");
+    *out = nullptr;
+    if (!p) return fail(VB_ERR_INVALID_ARG, "plan is null");
+    if (dtype != VB_DTYPE_F32 && dtype != VB_DTYPE_BF16 && dtype != VB_DTYPE_F16) return fail(VB_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+    if (p->n > 0 && !pointers) return fail(VB_ERR_INVALID_ARG, "pointers is null");
+    const int64_t size = dtype == VB_DTYPE_F32 ? 4 : 2, per16 = 16 / size;
+    std::unique_ptr<vb_ns_matrices> l(new vb_ns_matrices());
+    l->plan = p;
+    l->dtype = dtype;
+    l->arrays.resize((size_t)p->n);
+    l->vec.assign((size_t)p->n, 0);
+    std::vector<const void *> seen;
+    for (int64_t i = 0; i < p->n; ++i) {
+        const int64_t rows = p->rows[i], cols = p->cols[i];
+        if (rows == 0 || cols == 0) continue;
+        const int64_t sr = strides ? strides[2 * i] : cols, sc = strides ? strides[2 * i + 1] : 1;
+        if (sr < 0 || sc < 0) return fail(VB_ERR_INVALID_ARG, "matrix %lld has a negative stride", (long long)i);
+        if (sr > (INT64_MAX >> 22) || sc > (INT64_MAX >> 22)) return fail(VB_ERR_INVALID_ARG, "matrix %lld has strides out of range", (long long)i);
+        NsArray &a = l->arrays[(size_t)i];
+        a.ptr = pointers[i];
+        a.si = rows > cols ? sc : sr;  // the working matrix has the short side first
+        a.sj = rows > cols ? sr : sc;
+        if (!a.ptr) {
+            l->any_null = true;
+            continue;
+        }
+        const uintptr_t at = reinterpret_cast<uintptr_t>(a.ptr);
+        if (at % (uintptr_t)size) return fail(VB_ERR_INVALID_ARG, "pointer %lld is not aligned to its elements", (long long)i);
+        cudaPointerAttributes attr;
+        const cudaError_t err = cudaPointerGetAttributes(&attr, a.ptr);
+        if (err != cudaSuccess) {
+            cudaGetLastError();
+            return fail(VB_ERR_INVALID_ARG, "pointer %lld is not one CUDA knows: %s", (long long)i, cudaGetErrorString(err));
+        }
+        if (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged)
+            return fail(VB_ERR_INVALID_ARG, "pointer %lld is not device memory", (long long)i);
+        if (attr.type == cudaMemoryTypeDevice && attr.device != p->device)
+            return fail(VB_ERR_INVALID_ARG, "pointer %lld lives on device %d, the engine runs on device %d", (long long)i, attr.device, p->device);
+        // where a side is 1 its stride says nothing: the matrix is then contiguous along the other
+        const int64_t n = std::min(rows, cols), m = std::max(rows, cols);
+        if (n == 1 && a.sj == 1) a.si = round_up(m, per16);
+        if (m == 1) a.si = per16, a.sj = 1;
+        const int64_t across = a.sj == 1 ? a.si : a.si == 1 ? a.sj : 1;
+        l->vec[(size_t)i] = (a.sj == 1 || a.si == 1) && at % 16 == 0 && across % per16 == 0;
+        const bool apart = (a.sj >= 1 && a.si >= (m - 1) * a.sj + 1) || (a.si >= 1 && a.sj >= (n - 1) * a.si + 1) ||
+                           (n == 1 && (a.sj >= 1 || m == 1));
+        if (!apart) l->writable = false, l->why = "elements of a matrix share an address";
+        seen.push_back(a.ptr);
+    }
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) l->writable = false, l->why = "two matrices start at one address";
+    *out = l.release();
+    return VB_OK;
+    VB_NS_END
+}
+
+int vb_ns_matrices_destroy(vb_ns_matrices *l)
+{
+    delete l;
+    return VB_OK;
+}
+
+int vb_orthogonalize(vb_ns_plan *p, const vb_ns_matrices *inputs, const vb_ns_matrices *outputs)
+{
+    VB_NS_BEGIN
+    DeviceGuard guard;
+    VB_TRY(begin_call(p, &guard));
+    VB_TRY(check_list(p, inputs, "inputs", false, false));
+    VB_TRY(check_list(p, outputs, "outputs", true, false));
+    VB_TRY(check_alias(inputs, outputs, "input and output", true));
+    NsElementwise w = p->ew;
+    w.planes = p->planes;
+    w.eps = p->eps;
+    w.types[0] = inputs->dtype;
+    NsElementwise fin = w;
+    fin.types[0] = outputs->dtype;
+    return run_plan(p, w, fin, false, [&](int64_t i, NsMatrixArg &a, bool finish) {
+        const vb_ns_matrices *source = finish ? outputs : inputs;
+        a.a[0] = source->arrays[(size_t)i];
+        a.direct = source->vec[(size_t)i];
+        a.live = 1;
+        a.scale = 1.0f;
+    });
+    VB_NS_END
+}
+
+int vb_muon_multi_tensor_step(vb_ns_plan *p, const vb_muon_step_params *hp, const vb_ns_matrices *params,
+                              const vb_ns_matrices *grads, const vb_ns_matrices *velocities, const float *scales)
+{
+    VB_NS_BEGIN
+    DeviceGuard guard;
+    VB_TRY(begin_call(p, &guard));
+    if (!hp) return fail(VB_ERR_INVALID_ARG, "hp is null");
+    if (!std::isfinite(hp->lr) || !std::isfinite(hp->momentum) || !std::isfinite(hp->weight_decay))
+        return fail(VB_ERR_INVALID_ARG, "hyper-parameters must be finite");
+    VB_TRY(check_list(p, params, "params", true, false));
+    VB_TRY(check_list(p, grads, "grads", false, true));
+    VB_TRY(check_list(p, velocities, "velocities", true, false));
+    VB_TRY(check_alias(params, velocities, "parameter and velocity", false));
+    VB_TRY(check_alias(params, grads, "parameter and gradient", false));
+    VB_TRY(check_alias(velocities, grads, "velocity and gradient", false));
+    NsElementwise w = p->ew;
+    w.planes = p->planes;
+    w.eps = p->eps;
+    w.types[0] = grads->dtype;
+    w.types[1] = velocities->dtype;
+    w.types[2] = params->dtype;
+    w.momentum = hp->momentum;
+    w.nesterov = hp->nesterov != 0;
+    w.decay = (float)(1.0 - (double)hp->lr * (double)hp->weight_decay);
+    w.rate = hp->lr;
+    return run_plan(p, w, w, true, [&](int64_t i, NsMatrixArg &a, bool) {
+        const size_t k = (size_t)i;
+        a.a[0] = grads->arrays[k];
+        a.a[1] = velocities->arrays[k];
+        a.a[2] = params->arrays[k];
+        a.direct = (uint32_t)grads->vec[k] | (uint32_t)velocities->vec[k] << 1 | (uint32_t)params->vec[k] << 2;
+        a.live = grads->arrays[k].ptr != nullptr;
+        a.scale = scales ? scales[i] : 1.0f;
+    });
+    VB_NS_END
+}
+
+int vb_debug_ns_plan_withhold_loads(vb_ns_plan *p, uint32_t wait_limit)
+{
+    if (!p) return fail(VB_ERR_INVALID_ARG, "plan is null");
+    p->withhold = true;
+    p->wait_limit = wait_limit;
+    return VB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,112 @@
+// Newton-Schulz on caller-owned matrices (include/volta_b200.h, "vb_ns_plan"): descriptors shared by
+// the planner (ns_plan.cu), the element-wise kernels (ns_gather.cu) and the tensor-core products
+// (ns_products.cu).
+//
+// Notation.  A matrix of r x c is worked on as X of n x m, n = min(r, c), m = max(r, c), transposed
+// where r > c.  Everything the tensor cores read is f16, in one plane (VB_NS_F16) or two whose sum
+// has 22 significand bits (VB_NS_F32_TC), zero-padded to multiples of 128 in both directions, and
+// stored times a power of two that the planner picks from bounds of the polynomials.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include "vb_internal.h"
+
+namespace vb {
+
+constexpr int kNsPad = 128;  // sides of the working matrices are multiples of this
+
+// One product of the iteration:  D = e E + f F + g sum_k A[m,k] B[n,k]
+// E and F (f16, leading dimension and planes of D; may be null) are read at D's position.
+enum NsProductFlags {
+    NS_B_MN_MAJOR = 1,  // B is stored [k][n] (the working matrix X); otherwise [n][k]
+};
+struct alignas(128) NsProduct {
+    CUtensorMap map_a;  // [rows][k], 64 x 128 boxes
+    CUtensorMap map_b;  // the same, or the 3-D view of [k][n] (see make_ns_map)
+    const __half *E, *F;
+    __half *D;
+    int32_t M, N, K;         // padded extents
+    int32_t ld;              // of D, E, F
+    int32_t plane_rows_a, plane_rows_b;  // rows between the planes of an operand
+    int64_t plane_d;         // elements between the planes of D, E, F
+    float e, f, g;
+    int32_t scale_power;     // e, f, g are multiplied by scale^scale_power (0, 1 or 2)
+    const float *scale;      // the matrix's normalisation (null where scale_power is 0)
+    int32_t matrix;          // index into the activity words
+    int32_t flags;
+};
+struct NsTile {
+    int32_t problem, m0, n0;
+    int32_t mirror;  // symmetric product: the tile is also stored transposed
+};
+
+struct NsLaunch {
+    const NsProduct *problems;
+    const NsTile *tiles;
+    int n_tiles;
+};
+
+// tile shapes of the product kernel
+enum NsTileShape {
+    NS_TILE_PAIR_256 = 0,  // two CTAs, 256 x 256
+    NS_TILE_128 = 1        // one CTA, 128 x 128
+};
+void ns_tile_extent(int shape, int *bm, int *bn);
+// Where a kernel reports a wait that ran out: a device word later kernels look at, a mapped one for the host.
+struct NsError {
+    uint32_t *device, *host;
+};
+// withhold: test hook, the producers stage nothing so that every wait runs out
+int launch_ns_products(const NsLaunch &launch, int shape, int planes, const uint32_t *d_active, NsError error,
+                       int sm_count, cudaStream_t stream, uint32_t wait_limit, bool withhold);
+int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, bool mn_major);
+
+// ---- element-wise kernels over the caller's matrices ---------------------------------------
+// A caller's array of one matrix in the working orientation: element (i, j) of X is at
+// ptr[i * si + j * sj].
+struct NsArray {
+    void *ptr;
+    int64_t si, sj;
+};
+constexpr int kNsBatch = 96;  // matrices of one element-wise launch (bounded by its parameter space)
+struct NsMatrixArg {
+    NsArray a[3];   // orthogonalize: input or output; step: gradient, velocity, parameter
+    float scale;    // step: s_i of the update
+    uint32_t live;  // 0: no gradient, the matrix is left alone
+    uint32_t direct; // bit k: array k has sj == 1 and rows on 16-byte boundaries
+};
+struct NsMatrixDims {
+    int32_t n, m;            // extents
+    int32_t np, mp;          // padded
+    int64_t x_off;           // element offset of the working matrix (plane 0)
+    int64_t final_off;       // the same of the last iterate
+    float final_scale;       // a stored value of the last iterate times this is the value
+    int32_t tile0, n_tiles;  // element-wise tiles of this matrix
+};
+struct NsElementwise {
+    const NsMatrixDims *dims;  // of every matrix of the plan
+    double *partials;          // one sum of squares per tile
+    float *scale;              // per matrix: X = scale * working matrix
+    uint32_t *active;          // per matrix: 0 = skipped by the products and by what follows
+    const uint32_t *error;     // set once a product kernel gave up a wait: nothing more is stored
+    __half *x;                 // working matrices
+    int planes;
+    int types[3];              // vb_dtype of the arrays of NsMatrixArg
+    float eps;
+    float momentum, decay, rate;
+    int nesterov;
+};
+struct NsBatchArgs {
+    NsMatrixArg m[kNsBatch];
+    int32_t first;  // index of m[0] in the plan
+    int32_t count;
+    int32_t tile0, n_tiles;
+};
+constexpr int kNsTileI = 64, kNsTileJ = 128;  // an element-wise tile of the working matrix
+int launch_ns_norm(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
+int launch_ns_gather(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
+int launch_ns_finish(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
+
+}  // namespace vb
