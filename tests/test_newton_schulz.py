@@ -80,9 +80,11 @@ def test_planned_products_are_the_iteration(shape, coefficients):
 
 
 def test_groups_follow_the_amplification_limits():
-    """Long matrices: the quintic runs in groups of 3 and 2, square ones step by step, the cubic as one."""
+    """Long matrices: the quintic runs in groups of 3 and 2 (of 2, 2 and 1 where the short side is small), square
+    ones step by step, the cubic as one."""
     grams = lambda shape, co: [p["stage"] for p in _products(*shape, co)[0] if p["gram"]]  # noqa: E731
-    assert len(grams((64, 256), QUINTIC)) == 2
+    assert len(grams((1024, 256), QUINTIC)) == 2
+    assert len(grams((64, 256), QUINTIC)) == 3
     assert len(grams((64, 64), QUINTIC)) == 5
     assert len(grams((256, 64), CUBIC)) == 1
 

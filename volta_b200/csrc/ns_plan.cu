@@ -12,10 +12,11 @@
 // further one of a group 4 n^3.  What limits a group is rounding: noise of size d in G (2^-12 |G|_F
 // spread over the spectrum) grows by the slope of t q(t)^2 with every step and reaches small eigenvalues'
 // q after k steps as d prod a^2.  In f16 the 1024-sided quintic run as one group is wrong by 10 to
-// 100 % on gradients with a decaying spectrum.  The first group of a call may amplify 150-fold (its Gram has
-// trace 1, so d is small), later ones, whose Gram is near the identity, 17-fold: with these limits
-// the error equals that of one step at a time (1e-3 to 4e-3 relative) on Gaussian, low-rank-plus-noise
-// and power-law spectra.  For the usual quintic this means groups of 3 and 2.  Matrices whose long
+// 100 % on gradients with a decaying spectrum.  The first group of a call may amplify 150-fold where
+// n >= 256 (its Gram has trace 1, and d falls with sqrt(n): less for smaller n), later ones, whose Gram is
+// near the identity, 17-fold: with these limits the error equals that of one step at a time (1e-3 to 4e-3
+// relative) on Gaussian, low-rank-plus-noise and power-law spectra.  For the usual quintic this means groups
+// of 3 and 2.  Matrices whose long
 // side is less than 1.5 times the short one run one step at a time: grouping saves nothing there.
 //
 // Powers of two.  Every stored matrix carries 2^e with e from the largest value its polynomial takes
@@ -68,7 +69,7 @@ int exponent_for(double bound)
     return std::min(e, 40);
 }
 
-std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, bool grouped)
+std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, double first_gain)
 {
     std::vector<std::vector<int>> groups;
     std::vector<double> lam(4097);
@@ -76,7 +77,7 @@ std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, bool g
     double gain = 1.0;
     for (int k = 0; k < (int)steps.size(); ++k) {
         const Step &s = steps[(size_t)k];
-        const bool fits = grouped && !groups.empty() && gain <= (groups.size() == 1 ? kFirstGroupGain : kGroupGain);
+        const bool fits = !groups.empty() && gain <= (groups.size() == 1 ? first_gain : std::min(first_gain, kGroupGain));
         if (!fits) {
             groups.emplace_back();
             gain = 1.0;
@@ -96,9 +97,9 @@ std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, bool g
 }
 
 // Returns false if the iterates leave the range that is sensible to hold.
-bool make_schedule(const std::vector<Step> &steps, bool grouped, Schedule *out)
+bool make_schedule(const std::vector<Step> &steps, double first_gain, Schedule *out)
 {
-    const auto groups = make_groups(steps, grouped);
+    const auto groups = make_groups(steps, first_gain);
     const int kSamples = 8192;
     std::vector<double> lam, sv;  // samples of the spectrum: of G, and the singular values of X
     for (int i = 0; i <= kSamples; ++i) lam.push_back((double)i / kSamples);
@@ -188,7 +189,13 @@ int read_steps(int n_steps, const float *coefficients, std::vector<Step> *steps)
     }
     return VB_OK;
 }
-bool runs_grouped(int64_t rows, int64_t cols) { return 2 * std::max(rows, cols) >= 3 * std::min(rows, cols); }
+// How much the first group of a matrix may amplify (0: one step at a time).
+double first_group_gain(int64_t rows, int64_t cols)
+{
+    const int64_t n = std::min(rows, cols), m = std::max(rows, cols);
+    if (2 * m < 3 * n) return 0.0;
+    return kFirstGroupGain * std::min(1.0, std::sqrt((double)n / 256.0));
+}
 
 struct Launch {
     NsLaunch l;
@@ -285,12 +292,10 @@ struct Carver {
 
 int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
 {
-    Schedule schedules[2];
-    for (int g = 0; g < 2; ++g)
-        if (!make_schedule(steps, g == 1, &schedules[g]))
-            return fail(VB_ERR_INVALID_ARG, kDivergedText);
     const int64_t n = p->n;
-    std::vector<int> kind((size_t)n);
+    std::vector<Schedule> schedules;       // the different ones among the matrices
+    std::vector<std::vector<std::vector<int>>> groupings;
+    std::vector<size_t> kind((size_t)n);
     std::vector<int32_t> tile_matrix;
     std::vector<int64_t> square_off((size_t)n);
     int64_t x_total = 0, square_total = 0, tiles = 0, batch_elements = 0;
@@ -303,7 +308,16 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         if (d.n == 0) d.m = 0;
         d.np = (int32_t)round_up(d.n, kNsPad);
         d.mp = (int32_t)round_up(d.m, kNsPad);
-        kind[(size_t)i] = runs_grouped(d.n, d.m) ? 1 : 0;
+        const double gain = first_group_gain(d.n, d.m);
+        const auto groups = make_groups(steps, gain);
+        size_t which = 0;
+        while (which < groupings.size() && groupings[which] != groups) ++which;
+        if (which == groupings.size()) {
+            groupings.push_back(groups);
+            schedules.emplace_back();
+            if (!make_schedule(steps, gain, &schedules.back())) return fail(VB_ERR_INVALID_ARG, kDivergedText);
+        }
+        kind[(size_t)i] = which;
         const Schedule &s = schedules[kind[(size_t)i]];
         d.x_off = x_total;
         d.final_off = s.final_buffer;  // buffer number for now
@@ -523,7 +537,7 @@ int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *
     std::vector<Step> steps;
     VB_TRY(read_steps(n_steps, coefficients, &steps));
     Schedule s;
-    if (!make_schedule(steps, runs_grouped(rows, cols), &s)) return fail(VB_ERR_INVALID_ARG, kDivergedText);
+    if (!make_schedule(steps, first_group_gain(rows, cols), &s)) return fail(VB_ERR_INVALID_ARG, kDivergedText);
     int64_t k = 0;
     for (size_t stage = 0; stage < s.stages.size(); ++stage)
         for (const Product &p : s.stages[stage]) {

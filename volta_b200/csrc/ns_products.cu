@@ -19,6 +19,12 @@
 //   256 x 256 by a CTA pair (cta_group::2): half the operand traffic per FLOP; used when a launch
 //             has enough such tiles for the device
 //   128 x 128 by one CTA: four times as many tiles, for launches that would leave SMs idle
+// Two planes (f32 accuracy): the tensor core adds to its f32 accumulator with truncation, which over a long
+// contraction of positive terms (the Gram's diagonal) drifts by 2^-25 per addition: 1.7e-5 on the result
+// at n = 2048, one accumulator for the whole sum.  So an accumulator takes 128 of the contraction (24
+// additions), and the epilogue warps sum the pieces in registers, correctly rounded, while the next piece runs.
+// One plane needs none of that: 65536 / 16 additions drift by less than the operands' rounding.
+//
 // Every wait is bounded; a wait that runs out sets *error, later kernels of the call then store nothing.
 #include <cuda_fp16.h>
 #include <algorithm>
@@ -36,7 +42,8 @@ constexpr int UMMA_K = 16;
 constexpr int kBoxBytes = 64 * BK * 2;
 constexpr int kRows128Bytes = 128 * BK * 2;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + kEpiWarps * 32;
+constexpr int kFirstEpiWarp = 2;  // warp 0 produces, warp 1 issues
+constexpr int kThreads = (kFirstEpiWarp + kEpiWarps) * 32;
 constexpr int kStageRowBytes = 128;
 constexpr int kStageWarpBytes = 32 * kStageRowBytes;
 constexpr uint32_t kDefaultWaitLimit = 1u << 22;
@@ -49,6 +56,7 @@ struct Cfg {
     static constexpr int kPlaneBytes = 2 * kRows128Bytes;  // 128 rows of A, 128 rows of B
     static constexpr int kStageBytes = kPlanes * kPlaneBytes;
     static constexpr int kTmemCols = 2 * BN;
+    static constexpr int kChunkBlocks = kPlanes == 1 ? 1 << 20 : 128 / BK;  // k blocks one accumulator takes
 };
 
 struct alignas(8) Barriers {
@@ -122,9 +130,9 @@ __device__ __forceinline__ float2 unpack_half(uint32_t w)
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// f[] += c * (32 values at src, both planes)
-template <int kPlanes>
-__device__ __forceinline__ void add_term(float (&f)[32], float c, const __half *src, int64_t plane)
+// f[kAt ..] += c * (32 values at src, both planes)
+template <int kPlanes, int kSize>
+__device__ __forceinline__ void add_term(float (&f)[kSize], int kAt, float c, const __half *src, int64_t plane)
 {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -143,13 +151,13 @@ __device__ __forceinline__ void add_term(float (&f)[32], float c, const __half *
                 x.x += y.x;
                 x.y += y.y;
             }
-            f[g * 8 + 2 * h] = fmaf(c, x.x, f[g * 8 + 2 * h]);
-            f[g * 8 + 2 * h + 1] = fmaf(c, x.y, f[g * 8 + 2 * h + 1]);
+            f[kAt + g * 8 + 2 * h] = fmaf(c, x.x, f[kAt + g * 8 + 2 * h]);
+            f[kAt + g * 8 + 2 * h + 1] = fmaf(c, x.y, f[kAt + g * 8 + 2 * h + 1]);
         }
     }
 }
 
-// Drains kCols columns of 32 accumulator rows.  A lane owns one row (TMEM lane = row); row-major stores
+// Drains kCols columns of 32 accumulator rows (kPlanes == 2: finished values, see the epilogue).  A lane owns one row (TMEM lane = row); row-major stores
 // go through the warp's staging buffer so that the warp writes 8 whole 128-byte lines per
 // instruction (16-byte pieces of row r sit at position piece ^ (r & 7): no bank conflicts either way).
 // Mirrored stores are contiguous along the rows the lanes hold: 64 bytes per instruction.
@@ -158,69 +166,70 @@ __device__ __forceinline__ void drain(uint32_t taddr, const NsProduct *p, int ro
                                       int lane, uint32_t stage)
 {
     const int64_t ld = p->ld, plane = p->plane_d;
-    const int64_t at = (int64_t)(row0 + lane) * ld + col0;
-    const __half *E = p->E, *F = p->F;
     __half *D = p->D;
-    const float ce = p->e * mult, cf = p->f * mult, cg = p->g * mult;
     const int r_sub = lane >> 2, seg = lane & 3;
     const uint32_t my_row = stage + (uint32_t)(lane * kStageRowBytes), my_sw = (uint32_t)(lane & 7);
     const uint32_t rd_row = stage + (uint32_t)(r_sub * kStageRowBytes);
     const uint32_t rd_c0 = (uint32_t)(((2 * seg) ^ r_sub) << 4), rd_c1 = (uint32_t)(((2 * seg + 1) ^ r_sub) << 4);
-    uint32_t low[2][16];  // second plane of the two pieces of a line
-#pragma unroll
+#pragma unroll(kPlanes == 2 ? 1 : kCols / 32)
     for (int cc = 0; cc < kCols / 32; ++cc) {
         uint32_t v[32];
-        tmem_ld_32x32_sync(taddr + (uint32_t)(cc * 32), v);
         float f[32];
+        tmem_ld_32x32_sync(taddr + (uint32_t)(cc * 32), v);
+        const float cg = kPlanes == 2 ? 1.0f : p->g * mult;
 #pragma unroll
         for (int j = 0; j < 32; ++j) f[j] = cg * __uint_as_float(v[j]);
-        if (E != nullptr) add_term<kPlanes>(f, ce, E + at + cc * 32, plane);
-        if (F != nullptr) add_term<kPlanes>(f, cf, F + at + cc * 32, plane);
-        uint32_t high[16];
+        if (kPlanes == 1) {
+            const int64_t at = (int64_t)(row0 + lane) * ld + col0 + cc * 32;
+            if (p->E != nullptr) add_term<1>(f, 0, p->e * mult, p->E + at, 0);
+            if (p->F != nullptr) add_term<1>(f, 0, p->f * mult, p->F + at, 0);
+        }
+        uint32_t high[16], low[kPlanes == 2 ? 16 : 1];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             high[j] = pack_half(f[2 * j], f[2 * j + 1]);
             if (kPlanes == 2) {  // what the first rounding left over (the difference is exact)
                 const float2 h = unpack_half(high[j]);
-                low[cc & 1][j] = pack_half(f[2 * j] - h.x, f[2 * j + 1] - h.y);
+                low[kPlanes == 2 ? j : 0] = pack_half(f[2 * j] - h.x, f[2 * j + 1] - h.y);
             }
         }
         if (mirror) {
             unsigned short *t = reinterpret_cast<unsigned short *>(D) + (int64_t)(col0 + cc * 32) * ld + row0 + lane;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-                t[(int64_t)j * ld] = (unsigned short)(j & 1 ? high[j >> 1] >> 16 : high[j >> 1] & 0xffffu);
-                if (kPlanes == 2)
-                    t[(int64_t)j * ld + plane] =
-                        (unsigned short)(j & 1 ? low[cc & 1][j >> 1] >> 16 : low[cc & 1][j >> 1] & 0xffffu);
+                *t = (unsigned short)(j & 1 ? high[j >> 1] >> 16 : high[j >> 1] & 0xffffu);
+                if (kPlanes == 2) {
+                    const uint32_t w = low[kPlanes == 2 ? j >> 1 : 0];
+                    t[plane] = (unsigned short)(j & 1 ? w >> 16 : w & 0xffffu);
+                }
+                t += ld;
+                asm volatile("" : "+l"(t));  // one running address: 32 of them kept across the pieces cost 64 registers
             }
         }
+        // one plane: two pieces make a 128-byte line of a row; two planes: a piece's 64 bytes of each
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            st_shared_128(my_row + ((((uint32_t)((cc & 1) * 4 + q)) ^ my_sw) << 4), high[4 * q], high[4 * q + 1],
-                          high[4 * q + 2], high[4 * q + 3]);
-        if (cc & 1) {  // 64 columns = one 128-byte line per row
+            st_shared_128(my_row + ((((uint32_t)((kPlanes == 1 ? (cc & 1) * 4 : 0) + q)) ^ my_sw) << 4), high[4 * q],
+                          high[4 * q + 1], high[4 * q + 2], high[4 * q + 3]);
+        if (kPlanes == 2) {
 #pragma unroll
-            for (int pl = 0; pl < kPlanes; ++pl) {
-                if (pl == 1) {
+            for (int q = 0; q < 4; ++q)
+                st_shared_128(my_row + ((((uint32_t)(4 + q)) ^ my_sw) << 4), low[(kPlanes == 2 ? 4 * q : 0)],
+                              low[kPlanes == 2 ? 4 * q + 1 : 0], low[kPlanes == 2 ? 4 * q + 2 : 0], low[kPlanes == 2 ? 4 * q + 3 : 0]);
+        }
+        if (kPlanes == 2 || (cc & 1)) {
+            __syncwarp();
 #pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        st_shared_128(my_row + ((((uint32_t)q) ^ my_sw) << 4), low[q >> 2][4 * (q & 3)],
-                                      low[q >> 2][4 * (q & 3) + 1], low[q >> 2][4 * (q & 3) + 2],
-                                      low[q >> 2][4 * (q & 3) + 3]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int pass = 0; pass < 4; ++pass) {
-                    uint32_t q[8];
-                    const uint32_t src = rd_row + (uint32_t)(pass * 8 * kStageRowBytes);
-                    ld_shared_128(src + rd_c0, q[0], q[1], q[2], q[3]);
-                    ld_shared_128(src + rd_c1, q[4], q[5], q[6], q[7]);
-                    st_global_256(D + pl * plane + (int64_t)(row0 + r_sub + 8 * pass) * ld + col0 + (cc - 1) * 32 +
-                                      seg * 16, q);
-                }
-                __syncwarp();
+            for (int pass = 0; pass < 4; ++pass) {
+                uint32_t q[8];
+                const uint32_t src = rd_row + (uint32_t)(pass * 8 * kStageRowBytes);
+                ld_shared_128(src + rd_c0, q[0], q[1], q[2], q[3]);
+                ld_shared_128(src + rd_c1, q[4], q[5], q[6], q[7]);
+                const int64_t row_at = (int64_t)(row0 + r_sub + 8 * pass) * ld + col0;
+                if (kPlanes == 1) st_global_256(D + row_at + (cc - 1) * 32 + seg * 16, q);
+                else st_global_256(D + (seg >> 1) * plane + row_at + cc * 32 + (seg & 1) * 16, q);
             }
+            __syncwarp();
         }
     }
 }
@@ -352,40 +361,43 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 next = fetch_tile(launch, active, t + n_groups);
                 if (ti.skipped) continue;
                 const uint32_t idesc = make_idesc(ti.b_mn, BM * kCtas, C::BN);
-                if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, wait_limit)) {
-                    ok = false;
-                    break;
-                }
-                tcgen05_fence_after();
-                const uint32_t tmem_d = tmem_base + (uint32_t)(acc * C::BN);
-                for (int kb = 0; kb < ti.k_blocks; ++kb) {
-                    if (!mbar_wait(&bars->full[stage], phase, abort_flag, wait_limit)) {
+                for (int k0 = 0; k0 < ti.k_blocks && ok; k0 += C::kChunkBlocks) {
+                    const int k1 = min(k0 + C::kChunkBlocks, ti.k_blocks);
+                    if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, wait_limit)) {
                         ok = false;
                         break;
                     }
                     tcgen05_fence_after();
-                    const uint32_t base = smem_u32(smem + (size_t)stage * C::kStageBytes);
-                    // two planes: three products, smallest first; the dropped low x low is below 2^-22
+                    const uint32_t tmem_d = tmem_base + (uint32_t)(acc * C::BN);
+                    for (int kb = k0; kb < k1; ++kb) {
+                        if (!mbar_wait(&bars->full[stage], phase, abort_flag, wait_limit)) {
+                            ok = false;
+                            break;
+                        }
+                        tcgen05_fence_after();
+                        const uint32_t base = smem_u32(smem + (size_t)stage * C::kStageBytes);
+                        // two planes: three products, smallest first; the dropped low x low is below 2^-22
 #pragma unroll
-                    for (int term = 0; term < (kPlanes == 2 ? 3 : 1); ++term) {
-                        const uint32_t sa = base + (kPlanes == 2 && term == 1 ? C::kPlaneBytes : 0);
-                        const uint32_t sb = base + kRows128Bytes + (kPlanes == 2 && term == 0 ? C::kPlaneBytes : 0);
+                        for (int term = 0; term < (kPlanes == 2 ? 3 : 1); ++term) {
+                            const uint32_t sa = base + (kPlanes == 2 && term == 1 ? C::kPlaneBytes : 0);
+                            const uint32_t sb = base + kRows128Bytes + (kPlanes == 2 && term == 0 ? C::kPlaneBytes : 0);
 #pragma unroll
-                        for (int kk = 0; kk < BK / UMMA_K; ++kk)
-                            tcgen05_mma_bf16<kCtas>(tmem_d, operand_desc(sa, false, kk), operand_desc(sb, ti.b_mn, kk),
-                                                    idesc, (kb > 0 || term > 0 || kk > 0) ? 1u : 0u);
+                            for (int kk = 0; kk < BK / UMMA_K; ++kk)
+                                tcgen05_mma_bf16<kCtas>(tmem_d, operand_desc(sa, false, kk), operand_desc(sb, ti.b_mn, kk),
+                                                        idesc, (kb > k0 || term > 0 || kk > 0) ? 1u : 0u);
+                        }
+                        tcgen05_commit<kCtas>(&bars->empty[stage]);
+                        if (++stage == C::kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
-                    tcgen05_commit<kCtas>(&bars->empty[stage]);
-                    if (++stage == C::kStages) {
-                        stage = 0;
-                        phase ^= 1u;
+                    if (!ok) break;
+                    tcgen05_commit<kCtas>(&bars->tmem_full[acc]);
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1u;
                     }
-                }
-                if (!ok) break;
-                tcgen05_commit<kCtas>(&bars->tmem_full[acc]);
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
                 }
             }
             if (!ok) {
@@ -394,11 +406,11 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             }
         }
         __syncwarp();
-    } else {
+    } else if (warp >= kFirstEpiWarp) {
         // ---- epilogue: warp w reads TMEM lane quarter w % 4 and half of the columns ----
         constexpr int kCols = C::BN / 2;
-        const int quarter = warp & 3, col_half = (warp - 2) >> 2;
-        const uint32_t my_stage = smem_u32(epi_stage) + (uint32_t)((warp - 2) * kStageWarpBytes);
+        const int quarter = warp & 3, col_half = (warp - kFirstEpiWarp) >> 2;
+        const uint32_t my_stage = smem_u32(epi_stage) + (uint32_t)((warp - kFirstEpiWarp) * kStageWarpBytes);
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -413,26 +425,73 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 mult = *p->scale;
                 if (p->scale_power == 2) mult *= mult;
             }
-            if (!__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[acc], acc_phase, abort_flag, wait_limit))) {
-                ok = false;
-                break;
-            }
-            tcgen05_fence_after();
             const int row0 = ti.m0 + (int)cta_rank * BM + quarter * 32;
             const int col0 = ti.n0 + col_half * kCols;
-            if (row0 < p->M && col0 < p->N)  // extents are multiples of 128: a warp's piece is all in or all out
-                drain<kPlanes, kCols>(tmem_base + ((uint32_t)(quarter * 32) << 16) +
-                                          (uint32_t)(acc * C::BN + col_half * kCols),
-                                      p, row0, col0, ti.mirror, mult, lane, my_stage);
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (kCtas == 2) mbar_remote_arrive(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
-                else mbar_arrive(&bars->tmem_empty[acc]);
+            // extents are multiples of 128: a warp's piece is all in or all out
+            const bool inside = row0 < p->M && col0 < p->N;
+            float sum[kPlanes == 2 ? kCols : 1];
+            if (kPlanes == 2) {  // the polynomial's other terms first: their loads overlap the first products
+                const int64_t at = (int64_t)(row0 + lane) * p->ld + col0;
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sum[kPlanes == 2 ? j : 0] = 0.0f;
+                if (inside && p->E != nullptr) {
+#pragma unroll
+                    for (int cc = 0; cc < kCols / 32; ++cc) {
+                        add_term<2>(sum, kPlanes == 2 ? cc * 32 : 0, p->e * mult, p->E + at + cc * 32, p->plane_d);
+                        asm volatile("" ::: "memory");  // no more than a piece's loads in registers at once
+                    }
+                }
+                if (inside && p->F != nullptr) {
+#pragma unroll
+                    for (int cc = 0; cc < kCols / 32; ++cc) {
+                        add_term<2>(sum, kPlanes == 2 ? cc * 32 : 0, p->f * mult, p->F + at + cc * 32, p->plane_d);
+                        asm volatile("" ::: "memory");
+                    }
+                }
             }
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
+            const float cg = p->g * mult;
+            for (int k0 = 0; k0 < ti.k_blocks && ok; k0 += C::kChunkBlocks) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[acc], acc_phase, abort_flag, wait_limit))) {
+                    ok = false;
+                    break;
+                }
+                tcgen05_fence_after();
+                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * C::BN + col_half * kCols);
+                if (kPlanes == 1) {
+                    if (inside) drain<kPlanes, kCols>(taddr, p, row0, col0, ti.mirror, mult, lane, my_stage);
+                } else {
+#pragma unroll
+                    for (int cc = 0; cc < kCols / 32; ++cc) {
+                        uint32_t v[32];
+                        tmem_ld_32x32_sync(taddr + (uint32_t)(cc * 32), v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            sum[kPlanes == 2 ? cc * 32 + j : 0] =
+                                fmaf(cg, __uint_as_float(v[j]), sum[kPlanes == 2 ? cc * 32 + j : 0]);
+                    }
+                    if (k0 + C::kChunkBlocks >= ti.k_blocks && inside) {
+                        // finished: back into this warp's part of the accumulator, drained from there piece by piece
+#pragma unroll
+                        for (int cc = 0; cc < kCols / 32; ++cc) {
+                            uint32_t v[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[kPlanes == 2 ? cc * 32 + j : 0]);
+                            tmem_st_32x32(taddr + (uint32_t)(cc * 32), v);
+                        }
+                        tmem_st_wait();
+                        drain<kPlanes, kCols>(taddr, p, row0, col0, ti.mirror, mult, lane, my_stage);
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (kCtas == 2) mbar_remote_arrive(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
+                    else mbar_arrive(&bars->tmem_empty[acc]);
+                }
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
             }
         }
         if (!ok && lane == 0) {
