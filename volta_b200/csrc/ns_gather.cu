@@ -243,7 +243,10 @@ ns_gather_kernel(const NsElementwise w, const __grid_constant__ NsBatchArgs b, c
     const int matrix = tile_matrix[index];
     const NsMatrixArg &a = b.m[matrix - b.first];
     const NsMatrixDims d = w.dims[matrix];
-    if (index == d.tile0 && threadIdx.x == 0) w.active[matrix] = a.live;
+    if (index == d.tile0 && threadIdx.x == 0) {
+        w.active[matrix] = a.live;
+        w.stored[matrix] = 0u;
+    }
     if (a.live == 0u) return;
     const TileView t = tile_view(d, index);
 

@@ -37,6 +37,7 @@ constexpr int kSquares = 5;  // short-side matrices alive at once: G, T, R, P an
 constexpr int kMaxSteps = 64;
 constexpr int64_t kMaxSide = 65536;
 constexpr double kFirstGroupGain = 150.0, kGroupGain = 17.0;
+constexpr uint32_t kDefaultWaitLimit = 1u << 22;  // polls, about a second
 constexpr double kDiverged = 1048576.0;
 // norm and gather of a batch follow each other; a batch's arrays should stay in the 126 MB L2 in between
 constexpr int64_t kBatchElements = 8 << 20;
@@ -197,11 +198,6 @@ double first_group_gain(int64_t rows, int64_t cols)
     return kFirstGroupGain * std::min(1.0, std::sqrt((double)n / 256.0));
 }
 
-struct Launch {
-    NsLaunch l;
-    int shape;
-};
-
 struct DeviceGuard {  // runs the call on the engine's device and leaves the caller's current one as it was
     int before = -1;
     int enter(int device)
@@ -245,7 +241,8 @@ struct vb_ns_plan {
     char *d_base = nullptr;  // one allocation: everything below lies in it
     vb::NsElementwise ew{};  // device pointers of the element-wise passes
     const int32_t *d_tile_matrix = nullptr;
-    std::vector<vb::Launch> launches;
+    vb::NsLaunch products{};
+    int shape = 0;
     struct Batch {
         int32_t first, count, tile0, n_tiles;
     };
@@ -253,7 +250,8 @@ struct vb_ns_plan {
     vb::NsError error{};
     uint32_t *h_error = nullptr;
     bool withhold = false;
-    uint32_t wait_limit = 0;
+    uint32_t wait_limit = 0;  // of the next call, 0: the default
+    uint32_t default_wait_limit = 0;
     std::unique_ptr<vb::NsBatchArgs> args;  // scratch of a call
 };
 
@@ -289,6 +287,45 @@ struct Carver {
         return p;
     }
 };
+
+// Calls fn(m0, n0, mirror) for every tile of a product that is computed; returns their number.
+template <typename Fn>
+uint32_t for_tiles(const NsProduct &pr, int shape, Fn &&fn)
+{
+    int bm, bn;
+    ns_tile_extent(shape, &bm, &bn);
+    const bool symmetric = (pr.flags & NS_B_MN_MAJOR) == 0;
+    uint32_t count = 0;
+    for (int m0 = 0; m0 < pr.M; m0 += bm)
+        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn, ++count) fn(m0, n0, symmetric && n0 > m0);
+    return count;
+}
+
+// The shape whose stages take less time if every stage is waited for: whole rounds of tiles over the
+// device's CTAs (pairs), a round costing its FLOPs per SM.  A 128 x 128 tile reads twice the
+// operands per FLOP and, with all SMs busy, runs at 0.6 of the pair's rate.
+int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t> &stage_begin, int sm_count)
+{
+    double cost[2] = {0.0, 0.0};
+    for (int shape = 0; shape < 2; ++shape) {
+        const double groups = shape == NS_TILE_PAIR_256 ? sm_count / 2 : sm_count;
+        const double tile = shape == NS_TILE_PAIR_256 ? 2.0 : 1.0 / 0.6;  // time of a tile per k
+        for (size_t k = 0; k + 1 < stage_begin.size(); ++k) {
+            double work = 0.0, longest = 0.0;
+            uint32_t tiles = 0;
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
+                const uint32_t count = for_tiles(problems[q], shape, [](int, int, bool) {});
+                tiles += count;
+                work += (double)count * problems[q].K;
+                longest = std::max(longest, (double)problems[q].K);
+            }
+            if (tiles == 0) continue;
+            const double rounds = std::ceil(tiles / groups), mean = work / tiles;
+            cost[shape] += tile * std::max(longest, rounds * mean);
+        }
+    }
+    return cost[NS_TILE_PAIR_256] <= cost[NS_TILE_128] ? NS_TILE_PAIR_256 : NS_TILE_128;
+}
 
 int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
 {
@@ -341,17 +378,12 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
     }
     for (auto &d : p->dims) d.final_off = d.x_off + (d.final_off == BUF_X1 ? x_total : 0);
 
-    // stages of all matrices side by side: launch k runs every matrix's k-th stage
-    struct HostLaunch {
-        std::vector<NsProduct> problems;
-        std::vector<NsTile> tiles;
-        int shape;
-    };
-    std::vector<HostLaunch> launches;
-    size_t n_launches = 0;
+    // stages of all matrices side by side: stage k of every matrix, then stage k + 1
+    size_t n_stages = 0;
     for (int64_t i = 0; i < n; ++i)
-        if (p->dims[(size_t)i].n > 0) n_launches = std::max(n_launches, schedules[kind[(size_t)i]].stages.size());
-    launches.resize(n_launches);
+        if (p->dims[(size_t)i].n > 0) n_stages = std::max(n_stages, schedules[kind[(size_t)i]].stages.size());
+    std::vector<NsProduct> problems;
+    std::vector<NsTile> tile_list;
 
     // The carving is done twice: for the size, then with the addresses (tensor maps need them).
     __half *x_base = nullptr, *square_base = nullptr;
@@ -364,21 +396,22 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         p->ew.partials = c.take<double>((size_t)tiles);
         p->ew.scale = c.take<float>((size_t)n);
         p->ew.active = c.take<uint32_t>((size_t)n);
+        p->ew.stored = c.take<uint32_t>((size_t)n);
         p->error.device = c.take<uint32_t>(1);
         p->ew.error = p->error.device;
         NsMatrixDims *d_dims = c.take<NsMatrixDims>((size_t)n);
         int32_t *d_tile_matrix = c.take<int32_t>(tile_matrix.size());
         p->ew.dims = d_dims;
         p->d_tile_matrix = d_tile_matrix;
-        for (size_t k = 0; k < n_launches; ++k) {
-            HostLaunch &hl = launches[k];
-            hl.problems.clear();
-            hl.tiles.clear();
+        problems.clear();
+        std::vector<size_t> stage_begin;  // of every stage's products in `problems`
+        for (size_t k = 0; k < n_stages; ++k) {
+            stage_begin.push_back(problems.size());
             for (int64_t i = 0; i < n; ++i) {
                 const NsMatrixDims &d = p->dims[(size_t)i];
                 const Schedule &s = schedules[kind[(size_t)i]];
                 if (d.n == 0 || k >= s.stages.size()) continue;
-                const int64_t xp = (int64_t)d.np * d.mp, sp = (int64_t)d.np * d.np;
+                const int64_t sp = (int64_t)d.np * d.np;
                 auto address = [&](int buffer) -> __half * {
                     if (buffer < 0) return nullptr;
                     if (buffer == BUF_X0) return x_base + d.x_off;
@@ -390,52 +423,59 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                     q.M = d.np;
                     q.N = pr.update ? d.mp : d.np;
                     q.K = pr.gram ? d.mp : d.np;
-                    q.ld = q.N;
-                    q.plane_rows_a = q.plane_rows_b = d.np;
-                    q.plane_d = pr.update ? xp : sp;
-                    q.E = address(pr.E);
-                    q.F = address(pr.F);
-                    q.D = address(pr.D);
-                    q.e = (float)pr.e, q.f = (float)pr.f, q.g = (float)pr.g;
+                    q.plane_rows = d.np;
+                    q.n_terms = pr.F >= 0 ? 2 : pr.E >= 0 ? 1 : 0;
+                    q.term[0] = (float)pr.e, q.term[1] = (float)pr.f, q.g = (float)pr.g;
                     q.scale_power = pr.scale_power;
                     q.scale = p->ew.scale + i;
                     q.matrix = (int32_t)i;
                     q.flags = pr.update ? NS_B_MN_MAJOR : 0;
                     if (round == 1) {
-                        VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, (int64_t)p->planes * d.np, false));
-                        VB_TRY(make_ns_map(&q.map_b, address(pr.B), pr.update ? q.N : q.K, (int64_t)p->planes * d.np, pr.update));
+                        const int64_t outer = (int64_t)p->planes * d.np;
+                        VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, outer, NS_MAP_ROWS));
+                        VB_TRY(make_ns_map(&q.map_b, address(pr.B), pr.update ? q.N : q.K, outer, pr.update ? NS_MAP_MN : NS_MAP_ROWS));
+                        if (pr.E >= 0) VB_TRY(make_ns_map(&q.map_term[0], address(pr.E), q.N, outer, NS_MAP_PIECE));
+                        if (pr.F >= 0) VB_TRY(make_ns_map(&q.map_term[1], address(pr.F), q.N, outer, NS_MAP_PIECE));
+                        VB_TRY(make_ns_map(&q.map_d, address(pr.D), q.N, outer, NS_MAP_PIECE));
+                        if (!pr.update) VB_TRY(make_ns_map(&q.map_mirror, address(pr.D), q.N, outer, NS_MAP_MIRROR));
                     }
-                    hl.problems.push_back(q);
+                    problems.push_back(q);
                 }
             }
-            // long contractions first: the tail of a launch is then made of short ones
-            std::stable_sort(hl.problems.begin(), hl.problems.end(), [](const NsProduct &a, const NsProduct &b) { return a.K > b.K; });
-            auto make_tiles = [&](int shape) {
-                int bm, bn;
-                ns_tile_extent(shape, &bm, &bn);
-                hl.tiles.clear();
-                hl.shape = shape;
-                for (size_t q = 0; q < hl.problems.size(); ++q) {
-                    const NsProduct &pr = hl.problems[q];
-                    const bool symmetric = (pr.flags & NS_B_MN_MAJOR) == 0;
-                    for (int m0 = 0; m0 < pr.M; m0 += bm)
-                        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn)
-                            hl.tiles.push_back({(int32_t)q, m0, n0, symmetric && n0 > m0 ? 1 : 0});
-                }
-            };
-            make_tiles(NS_TILE_PAIR_256);
-            if ((int)hl.tiles.size() < p->eng->sm_count / 2) make_tiles(NS_TILE_128);
-            NsProduct *d_problems = c.take<NsProduct>(hl.problems.size());
-            NsTile *d_tiles = c.take<NsTile>(hl.tiles.size());
-            if (round == 1) {
-                VB_CUDA(cudaMemcpyAsync(d_problems, hl.problems.data(), hl.problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
-                VB_CUDA(cudaMemcpyAsync(d_tiles, hl.tiles.data(), hl.tiles.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
-                p->launches.push_back({{d_problems, d_tiles, (int)hl.tiles.size()}, hl.shape});
-                int bm, bn;
-                ns_tile_extent(hl.shape, &bm, &bn);
-                for (const NsTile &t : hl.tiles)
-                    p->flops += 2.0 * (p->planes == 2 ? 3.0 : 1.0) * bm * bn * hl.problems[(size_t)t.problem].K;
+            // long contractions first: what is left at a stage's end is then short
+            std::stable_sort(problems.begin() + (ptrdiff_t)stage_begin.back(), problems.end(),
+                             [](const NsProduct &a, const NsProduct &b) { return a.K > b.K; });
+        }
+        stage_begin.push_back(problems.size());
+        p->shape = pick_shape(problems, stage_begin, p->eng->sm_count);
+        tile_list.clear();
+        std::vector<uint32_t> done((size_t)n, 0), stage_done((size_t)n, 0);
+        for (size_t k = 0; k < n_stages; ++k) {
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
+                const size_t i = (size_t)problems[q].matrix;
+                stage_done[i] += for_tiles(problems[q], p->shape, [&](int m0, int n0, bool mirror) {
+                    tile_list.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, done[i], 0});
+                });
             }
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) done[(size_t)problems[q].matrix] = stage_done[(size_t)problems[q].matrix];
+        }
+        NsProduct *d_problems = c.take<NsProduct>(problems.size());
+        NsTile *d_tiles = c.take<NsTile>(tile_list.size());
+        if (tile_list.size() > (size_t)INT32_MAX) return fail(VB_ERR_UNSUPPORTED, "the plan's products have too many tiles");
+        p->products = {d_problems, d_tiles, p->ew.stored, (int)tile_list.size()};
+        if (round == 1) {
+            VB_CUDA(cudaMemcpyAsync(d_problems, problems.data(), problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
+            VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
+            int bm, bn;
+            ns_tile_extent(p->shape, &bm, &bn);
+            double stage_flops = 0.0;
+            for (size_t q = 0; q < problems.size(); ++q)
+                stage_flops = std::max(stage_flops, 2.0 * (double)problems[q].M * problems[q].N * problems[q].K * 3.0);
+            // the default bound (about a second) plus two per 1e14 FLOPs of the largest product: a role may rightly
+            // wait for a whole stage
+            p->default_wait_limit = (uint32_t)std::min(1e9, kDefaultWaitLimit * (1.0 + 2.0 * std::floor(stage_flops / 1e14)));
+            for (const NsTile &t : tile_list)
+                p->flops += 2.0 * (p->planes == 2 ? 3.0 : 1.0) * bm * bn * problems[(size_t)t.problem].K;
         }
         if (round == 0) {
             p->workspace = c.used;
@@ -466,23 +506,28 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, const NsElementwise &fin, bo
         args.n_tiles = b.n_tiles;
         for (int32_t k = 0; k < b.count; ++k) fill(b.first + k, args.m[k], finish);
     };
+    prof_begin(e, VB_PHASE_MUON_PRE);
     for (const auto &b : p->batches) {
         load(b, false);
         VB_TRY(launch_ns_norm(w, args, p->d_tile_matrix, step, e->stream));
         VB_TRY(launch_ns_gather(w, args, p->d_tile_matrix, step, e->stream));
         if (b.n_tiles > 0) e->launches += 2;
     }
-    for (const Launch &l : p->launches) {
-        VB_TRY(launch_ns_products(l.l, l.shape, p->planes, w.active, p->error, e->sm_count, e->stream, p->wait_limit, p->withhold));
-        p->withhold = false;
-        p->wait_limit = 0;
-        if (l.l.n_tiles > 0) e->launches += 1;
-    }
+    prof_end(e, VB_PHASE_MUON_PRE);
+    prof_begin(e, VB_PHASE_MUON_NS);
+    VB_TRY(launch_ns_products(p->products, p->shape, p->planes, w.active, p->error, e->sm_count, e->stream,
+                              p->wait_limit ? p->wait_limit : p->default_wait_limit, p->withhold));
+    p->withhold = false;
+    p->wait_limit = 0;
+    if (p->products.n_tiles > 0) e->launches += 1;
+    prof_end(e, VB_PHASE_MUON_NS);
+    prof_begin(e, VB_PHASE_MUON_APPLY);
     for (const auto &b : p->batches) {
         load(b, true);
         VB_TRY(launch_ns_finish(fin, args, p->d_tile_matrix, step, e->stream));
         if (b.n_tiles > 0) e->launches += 1;
     }
+    prof_end(e, VB_PHASE_MUON_APPLY);
     return VB_OK;
 }
 

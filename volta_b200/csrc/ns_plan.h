@@ -23,15 +23,16 @@ enum NsProductFlags {
     NS_B_MN_MAJOR = 1,  // B is stored [k][n] (the working matrix X); otherwise [n][k]
 };
 struct alignas(128) NsProduct {
-    CUtensorMap map_a;  // [rows][k], 64 x 128 boxes
-    CUtensorMap map_b;  // the same, or the 3-D view of [k][n] (see make_ns_map)
-    const __half *E, *F;
-    __half *D;
-    int32_t M, N, K;         // padded extents
-    int32_t ld;              // of D, E, F
-    int32_t plane_rows_a, plane_rows_b;  // rows between the planes of an operand
-    int64_t plane_d;         // elements between the planes of D, E, F
-    float e, f, g;
+    // tensor maps, see make_ns_map
+    CUtensorMap map_a;         // operand, NS_MAP_ROWS
+    CUtensorMap map_b;         // operand, NS_MAP_ROWS or NS_MAP_MN
+    CUtensorMap map_term[2];   // E and F, NS_MAP_PIECE
+    CUtensorMap map_d;         // D, NS_MAP_PIECE
+    CUtensorMap map_mirror;    // D, NS_MAP_MIRROR
+    int32_t M, N, K;           // padded extents
+    int32_t plane_rows;        // rows between the planes of a matrix
+    int32_t n_terms;           // 0: D = g acc, 1: E, 2: E and F
+    float term[2], g;          // e, f, g
     int32_t scale_power;     // e, f, g are multiplied by scale^scale_power (0, 1 or 2)
     const float *scale;      // the matrix's normalisation (null where scale_power is 0)
     int32_t matrix;          // index into the activity words
@@ -39,16 +40,20 @@ struct alignas(128) NsProduct {
 };
 struct NsTile {
     int32_t problem, m0, n0;
-    int32_t mirror;  // symmetric product: the tile is also stored transposed
+    int32_t mirror;   // symmetric product: the tile is also stored transposed
+    uint32_t after;   // tiles of the matrix's earlier stages: all of them must be stored before this one starts
+    int32_t pad;
 };
 
+// The tiles of every stage of every matrix, earlier stages first.
 struct NsLaunch {
     const NsProduct *problems;
     const NsTile *tiles;
+    uint32_t *stored;  // per matrix: epilogue warps' arrivals, zeroed by the gather pass
     int n_tiles;
 };
 
-// tile shapes of the product kernel
+// Tile shapes of the product kernel.
 enum NsTileShape {
     NS_TILE_PAIR_256 = 0,  // two CTAs, 256 x 256
     NS_TILE_128 = 1        // one CTA, 128 x 128
@@ -61,7 +66,14 @@ struct NsError {
 // withhold: test hook, the producers stage nothing so that every wait runs out
 int launch_ns_products(const NsLaunch &launch, int shape, int planes, const uint32_t *d_active, NsError error,
                        int sm_count, cudaStream_t stream, uint32_t wait_limit, bool withhold);
-int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, bool mn_major);
+// A row-major f16 matrix [outer][inner] as the kernel moves it.
+enum NsMap {
+    NS_MAP_ROWS = 0,   // 64 x 128 boxes, 128-byte swizzle: 128 rows x 64 k of an operand
+    NS_MAP_MN = 1,     // 64 x 64 x 2 boxes of the view [inner / 64][outer][64], same swizzle: 64 k x 128 columns
+    NS_MAP_PIECE = 2,  // 64 x 32 boxes, same swizzle: what an epilogue warp reads or writes at once
+    NS_MAP_MIRROR = 3  // 32 x 64 boxes: the same piece transposed
+};
+int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int kind);
 
 // ---- element-wise kernels over the caller's matrices ---------------------------------------
 // A caller's array of one matrix in the working orientation: element (i, j) of X is at
@@ -90,6 +102,7 @@ struct NsElementwise {
     double *partials;          // one sum of squares per tile
     float *scale;              // per matrix: X = scale * working matrix
     uint32_t *active;          // per matrix: 0 = skipped by the products and by what follows
+    uint32_t *stored;          // per matrix: set to zero for the products
     const uint32_t *error;     // set once a product kernel gave up a wait: nothing more is stored
     __half *x;                 // working matrices
     int planes;

@@ -14,11 +14,27 @@
 // All sides are padded to 128 with zeros that reproduce themselves, so nothing is masked here except
 // the second half of a 256-row or 256-column tile at the edge.
 //
+// One persistent, cooperative launch runs all stages of all matrices: the tile list holds stage after
+// stage, every CTA (pair) walks its share in order, and a tile starts once all tiles of the same
+// matrix's earlier stages are stored (a counter per matrix; release by the storing warps, acquire by the
+// loading ones).  A tile waits only for tiles before it in the list and all CTAs are resident, so the first
+// unfinished tile can always run.  Against one launch per stage this saves the launches' fill and drain
+// (10 us a stage for a 256 x 784 matrix by itself) and lets other matrices' tiles fill the gaps between the
+// stages of one.
+//
 // Warp roles as in ns_gemm_tc.cu: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue with two
-// accumulators; a persistent grid walks the tile list.  Two shapes:
-//   256 x 256 by a CTA pair (cta_group::2): half the operand traffic per FLOP; used when a launch
-//             has enough such tiles for the device
-//   128 x 128 by one CTA: four times as many tiles, for launches that would leave SMs idle
+// accumulators.  Two shapes:
+//   256 x 256 by a CTA pair (cta_group::2): half the operand traffic per FLOP
+//   128 x 128 by one CTA: four times as many tiles, for lists that would leave SMs idle
+// (the planner picks, see pick_shape).
+//
+// Epilogue.  A warp owns 32 accumulator rows and takes them 64 columns at a time: TMEM -> registers, the
+// terms E and F from its own shared-memory buffer (fetched by TMA while the products run), rounding, D into
+// another buffer and from there by TMA to memory; the transposed piece of a symmetric product is built in a
+// third (neighbouring lanes exchange halves, so each lane writes words) and stored the same way.  With plain
+// loads and stores from registers (a lane per row) a 256 x 256 tile's epilogue took 10 to 13 thousand cycles
+// and a fence 3 thousand, against 8 thousand for the products at k = 1024: it, not the tensor core, set the pace.
+//
 // Two planes (f32 accuracy): the tensor core adds to its f32 accumulator with truncation, which over a long
 // contraction of positive terms (the Gram's diagonal) drifts by 2^-25 per addition: 1.7e-5 on the result
 // at n = 2048, one accumulator for the whole sum.  So an accumulator takes 128 of the contraction (24
@@ -44,15 +60,15 @@ constexpr int kRows128Bytes = 128 * BK * 2;
 constexpr int kEpiWarps = 8;
 constexpr int kFirstEpiWarp = 2;  // warp 0 produces, warp 1 issues
 constexpr int kThreads = (kFirstEpiWarp + kEpiWarps) * 32;
-constexpr int kStageRowBytes = 128;
-constexpr int kStageWarpBytes = 32 * kStageRowBytes;
-constexpr uint32_t kDefaultWaitLimit = 1u << 22;
-constexpr int kMaxStages = 6;
+constexpr int kPieceCols = 64;
+constexpr int kPieceBytes = 32 * kPieceCols * 2;  // 32 rows of 128 bytes, 16-byte parts of row r at part ^ (r & 7)
+constexpr int kEpiWarpBytes = 3 * kPieceBytes;    // term, result, mirrored result
+constexpr int kMaxStages = 4;
 
 template <int kCtas, int kPlanes>
 struct Cfg {
     static constexpr int BN = 128 * kCtas;
-    static constexpr int kStages = kPlanes == 1 ? 6 : 3;
+    static constexpr int kStages = kPlanes == 1 ? 4 : 2;
     static constexpr int kPlaneBytes = 2 * kRows128Bytes;  // 128 rows of A, 128 rows of B
     static constexpr int kStageBytes = kPlanes * kPlaneBytes;
     static constexpr int kTmemCols = 2 * BN;
@@ -64,6 +80,7 @@ struct alignas(8) Barriers {
     uint64_t empty[kMaxStages];
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
+    uint64_t term_full[kEpiWarps];
     uint32_t tmem_base;
     uint32_t abort;
     uint32_t skip;
@@ -72,7 +89,7 @@ template <int kCtas, int kPlanes>
 constexpr size_t smem_bytes()
 {
     using C = Cfg<kCtas, kPlanes>;
-    return 1024 + (size_t)C::kStages * C::kStageBytes + kEpiWarps * kStageWarpBytes + sizeof(Barriers);
+    return 1024 + (size_t)C::kStages * C::kStageBytes + kEpiWarps * kEpiWarpBytes + sizeof(Barriers);
 }
 static_assert(smem_bytes<2, 1>() <= 232448 && smem_bytes<1, 2>() <= 232448, "a CTA has 227 KiB of shared memory");
 
@@ -96,14 +113,16 @@ __device__ __forceinline__ uint32_t make_idesc(bool b_mn_major, int m, int n)
 
 struct Tile {
     const NsProduct *p;
-    int m0, n0, k_blocks;
+    int m0, n0, k_blocks, matrix;
+    uint32_t after;
     bool mirror, b_mn, skipped;
 };
 __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *active, int t)
 {
     Tile ti;
     ti.p = l.problems;
-    ti.m0 = ti.n0 = ti.k_blocks = 0;
+    ti.m0 = ti.n0 = ti.k_blocks = ti.matrix = 0;
+    ti.after = 0;
     ti.mirror = ti.b_mn = false;
     ti.skipped = true;
     if (t < l.n_tiles) {
@@ -113,11 +132,34 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
         ti.m0 = tile.m0;
         ti.n0 = tile.n0;
         ti.mirror = tile.mirror != 0;
+        ti.after = tile.after;
+        ti.matrix = p->matrix;
         ti.k_blocks = p->K / BK;
         ti.b_mn = (p->flags & NS_B_MN_MAJOR) != 0;
         ti.skipped = __ldcg(active + p->matrix) == 0u;
     }
     return ti;
+}
+
+__device__ __forceinline__ uint32_t load_acquire(const uint32_t *p)
+{
+    uint32_t v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+// Waits until the matrix's earlier stages are stored.  Bounded, and given up as soon as any CTA reported an error.
+__device__ __forceinline__ bool wait_stored(const uint32_t *counter, uint32_t target, const uint32_t *error,
+                                            volatile uint32_t *abort_flag, uint32_t wait_limit)
+{
+    if (target == 0u) return true;
+    for (uint32_t i = 0; i < wait_limit; ++i) {
+        if (load_acquire(counter) >= target) return true;
+        if ((i & 31u) == 31u) {
+            if (*abort_flag != 0u || *reinterpret_cast<const volatile uint32_t *>(error) != 0u) return false;
+            __nanosleep(64);
+        }
+    }
+    return false;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b)
@@ -130,109 +172,125 @@ __device__ __forceinline__ float2 unpack_half(uint32_t w)
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// f[kAt ..] += c * (32 values at src, both planes)
-template <int kPlanes, int kSize>
-__device__ __forceinline__ void add_term(float (&f)[kSize], int kAt, float c, const __half *src, int64_t plane)
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t smem_src, int c0, int c1)
 {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const uint4 q0 = reinterpret_cast<const uint4 *>(src)[g];
-        const uint32_t w0[4] = {q0.x, q0.y, q0.z, q0.w};
-        uint32_t w1[4] = {0u, 0u, 0u, 0u};
-        if (kPlanes == 2) {
-            const uint4 q1 = reinterpret_cast<const uint4 *>(src + plane)[g];
-            w1[0] = q1.x; w1[1] = q1.y; w1[2] = q1.z; w1[3] = q1.w;
-        }
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            float2 x = unpack_half(w0[h]);
-            if (kPlanes == 2) {
-                const float2 y = unpack_half(w1[h]);
-                x.x += y.x;
-                x.y += y.y;
-            }
-            f[kAt + g * 8 + 2 * h] = fmaf(c, x.x, f[kAt + g * 8 + 2 * h]);
-            f[kAt + g * 8 + 2 * h + 1] = fmaf(c, x.y, f[kAt + g * 8 + 2 * h + 1]);
-        }
-    }
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1), "r"(smem_src)
+                 : "memory");
 }
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// Drains kCols columns of 32 accumulator rows (kPlanes == 2: finished values, see the epilogue).  A lane owns one row (TMEM lane = row); row-major stores
-// go through the warp's staging buffer so that the warp writes 8 whole 128-byte lines per
-// instruction (16-byte pieces of row r sit at position piece ^ (r & 7): no bank conflicts either way).
-// Mirrored stores are contiguous along the rows the lanes hold: 64 bytes per instruction.
+// The warp's share of one tile: kCols columns of 32 rows.
 template <int kPlanes, int kCols>
-__device__ __forceinline__ void drain(uint32_t taddr, const NsProduct *p, int row0, int col0, bool mirror, float mult,
-                                      int lane, uint32_t stage)
-{
-    const int64_t ld = p->ld, plane = p->plane_d;
-    __half *D = p->D;
-    const int r_sub = lane >> 2, seg = lane & 3;
-    const uint32_t my_row = stage + (uint32_t)(lane * kStageRowBytes), my_sw = (uint32_t)(lane & 7);
-    const uint32_t rd_row = stage + (uint32_t)(r_sub * kStageRowBytes);
-    const uint32_t rd_c0 = (uint32_t)(((2 * seg) ^ r_sub) << 4), rd_c1 = (uint32_t)(((2 * seg + 1) ^ r_sub) << 4);
-#pragma unroll(kPlanes == 2 ? 1 : kCols / 32)
-    for (int cc = 0; cc < kCols / 32; ++cc) {
-        uint32_t v[32];
-        float f[32];
-        tmem_ld_32x32_sync(taddr + (uint32_t)(cc * 32), v);
-        const float cg = kPlanes == 2 ? 1.0f : p->g * mult;
+struct Drain {
+    const NsProduct *p;
+    uint8_t *buffers;     // this warp's
+    uint64_t *term_full;  // this warp's barrier
+    uint32_t &term_phase;
+    int row0, col0, lane;
+    int per_piece;        // loads of a piece: terms x planes
+    bool mirror;
+
+    // load `index` of the tile: piece by piece, E before F, plane 0 before plane 1
+    __device__ __forceinline__ void fetch(int index) const
+    {
+        if (lane != 0 || index >= per_piece * (kCols / kPieceCols)) return;
+        const int piece = index / per_piece, rest = index % per_piece;
+        mbar_expect_tx(term_full, kPieceBytes);
+        tma_load_2d<1>(buffers, &p->map_term[rest / kPlanes], col0 + piece * kPieceCols,
+                       row0 + (rest % kPlanes) * p->plane_rows, smem_u32(term_full));
+    }
+    // one plane of a finished piece: h[k] holds columns 2k and 2k + 1 of this lane's row
+    __device__ __forceinline__ void store(const uint32_t (&h)[32], int piece, int plane) const
+    {
+        if (lane == 0) bulk_wait_read();  // the stores before this one have left the buffers
+        __syncwarp();
+        const uint32_t out = smem_u32(buffers) + kPieceBytes, row = out + (uint32_t)(lane * 128);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = cg * __uint_as_float(v[j]);
-        if (kPlanes == 1) {
-            const int64_t at = (int64_t)(row0 + lane) * ld + col0 + cc * 32;
-            if (p->E != nullptr) add_term<1>(f, 0, p->e * mult, p->E + at, 0);
-            if (p->F != nullptr) add_term<1>(f, 0, p->f * mult, p->F + at, 0);
-        }
-        uint32_t high[16], low[kPlanes == 2 ? 16 : 1];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            high[j] = pack_half(f[2 * j], f[2 * j + 1]);
-            if (kPlanes == 2) {  // what the first rounding left over (the difference is exact)
-                const float2 h = unpack_half(high[j]);
-                low[kPlanes == 2 ? j : 0] = pack_half(f[2 * j] - h.x, f[2 * j + 1] - h.y);
-            }
-        }
+        for (int q = 0; q < 8; ++q)
+            st_shared_128(row + (uint32_t)((q ^ (lane & 7)) << 4), h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+        const uint32_t turned = out + kPieceBytes;
         if (mirror) {
-            unsigned short *t = reinterpret_cast<unsigned short *>(D) + (int64_t)(col0 + cc * 32) * ld + row0 + lane;
+            // column 2k (even lanes) or 2k + 1 (odd lanes), rows of a pair of lanes: 32 words of two 64-byte rows
+            const uint32_t word = turned + (uint32_t)((lane & 1) * 64 + (lane >> 1) * 4);
+            const uint32_t pick = (lane & 1) ? 0x3276u : 0x5410u;  // {other.hi, own.hi} or {own.lo, other.lo}
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                *t = (unsigned short)(j & 1 ? high[j >> 1] >> 16 : high[j >> 1] & 0xffffu);
-                if (kPlanes == 2) {
-                    const uint32_t w = low[kPlanes == 2 ? j >> 1 : 0];
-                    t[plane] = (unsigned short)(j & 1 ? w >> 16 : w & 0xffffu);
-                }
-                t += ld;
-                asm volatile("" : "+l"(t));  // one running address: 32 of them kept across the pieces cost 64 registers
+            for (int k = 0; k < 32; ++k) {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, h[k], 1);
+                const uint32_t w = __byte_perm(h[k], other, pick);
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(word + (uint32_t)(k * 128)), "r"(w) : "memory");
             }
         }
-        // one plane: two pieces make a 128-byte line of a row; two planes: a piece's 64 bytes of each
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            st_shared_128(my_row + ((((uint32_t)((kPlanes == 1 ? (cc & 1) * 4 : 0) + q)) ^ my_sw) << 4), high[4 * q],
-                          high[4 * q + 1], high[4 * q + 2], high[4 * q + 3]);
-        if (kPlanes == 2) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                st_shared_128(my_row + ((((uint32_t)(4 + q)) ^ my_sw) << 4), low[(kPlanes == 2 ? 4 * q : 0)],
-                              low[kPlanes == 2 ? 4 * q + 1 : 0], low[kPlanes == 2 ? 4 * q + 2 : 0], low[kPlanes == 2 ? 4 * q + 3 : 0]);
-        }
-        if (kPlanes == 2 || (cc & 1)) {
-            __syncwarp();
-#pragma unroll
-            for (int pass = 0; pass < 4; ++pass) {
-                uint32_t q[8];
-                const uint32_t src = rd_row + (uint32_t)(pass * 8 * kStageRowBytes);
-                ld_shared_128(src + rd_c0, q[0], q[1], q[2], q[3]);
-                ld_shared_128(src + rd_c1, q[4], q[5], q[6], q[7]);
-                const int64_t row_at = (int64_t)(row0 + r_sub + 8 * pass) * ld + col0;
-                if (kPlanes == 1) st_global_256(D + row_at + (cc - 1) * 32 + seg * 16, q);
-                else st_global_256(D + (seg >> 1) * plane + row_at + cc * 32 + (seg & 1) * 16, q);
-            }
-            __syncwarp();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            const int c = col0 + piece * kPieceCols, off = plane * p->plane_rows;
+            tma_store_2d(&p->map_d, out, c, row0 + off);
+            if (mirror) tma_store_2d(&p->map_mirror, turned, row0, c + off);
+            bulk_commit();
         }
     }
-}
+    // Returns false if a term did not arrive.  `drained` is called once the accumulator has been read.
+    template <typename Fn>
+    __device__ __forceinline__ bool run(uint32_t taddr, float mult, volatile uint32_t *abort_flag, uint32_t wait_limit,
+                                        Fn &&drained)
+    {
+        const float cg = p->g * mult;
+        int index = 0;  // of the load to wait for
+#pragma unroll 1
+        for (int piece = 0; piece < kCols / kPieceCols; ++piece) {
+            float f[kPieceCols];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t v[32];
+                tmem_ld_32x32_sync(taddr + (uint32_t)(piece * kPieceCols + half * 32), v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[half * 32 + j] = cg * __uint_as_float(v[j]);
+            }
+            if (piece + 1 == kCols / kPieceCols) drained();
+#pragma unroll 1
+            for (int r = 0; r < per_piece; ++r) {
+                if (!__all_sync(0xffffffffu, mbar_wait(term_full, term_phase, abort_flag, wait_limit))) return false;
+                term_phase ^= 1u;
+                const float c = p->term[r / kPlanes] * mult;
+                const uint32_t row = smem_u32(buffers) + (uint32_t)(lane * 128);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    uint32_t w[4];
+                    ld_shared_128(row + (uint32_t)((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 x = unpack_half(w[k]);
+                        f[q * 8 + 2 * k] = fmaf(c, x.x, f[q * 8 + 2 * k]);
+                        f[q * 8 + 2 * k + 1] = fmaf(c, x.y, f[q * 8 + 2 * k + 1]);
+                    }
+                }
+                __syncwarp();
+                fetch(++index);
+            }
+            uint32_t h[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                h[k] = pack_half(f[2 * k], f[2 * k + 1]);
+                if (kPlanes == 2) {  // what the rounding left over (the difference is exact)
+                    const float2 x = unpack_half(h[k]);
+                    f[2 * k] -= x.x;
+                    f[2 * k + 1] -= x.y;
+                }
+            }
+            store(h, piece, 0);
+            if (kPlanes == 2) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) h[k] = pack_half(f[2 * k], f[2 * k + 1]);
+                store(h, piece, 1);
+            }
+        }
+        return true;
+    }
+};
 
 // which role gave up: 1 producer, 2 MMA issuer, 3 epilogue
 __device__ __forceinline__ void report(const NsError &error, uint32_t role)
@@ -251,7 +309,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *epi_stage = smem + (size_t)C::kStages * C::kStageBytes;
-    Barriers *bars = reinterpret_cast<Barriers *>(epi_stage + kEpiWarps * kStageWarpBytes);
+    Barriers *bars = reinterpret_cast<Barriers *>(epi_stage + kEpiWarps * kEpiWarpBytes);
     volatile uint32_t *abort_flag = &bars->abort;
 
     const int warp = threadIdx.x >> 5;
@@ -260,6 +318,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     const int group_id = blockIdx.x / kCtas;
     const int n_groups = gridDim.x / kCtas;
     int n_tiles = launch.n_tiles;
+    constexpr uint32_t kArrivals = kCtas * kEpiWarps;  // on a matrix's counter, per tile
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
@@ -270,6 +329,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             mbar_init(&bars->tmem_full[a], 1);
             mbar_init(&bars->tmem_empty[a], kCtas * kEpiWarps);
         }
+        for (int w = 0; w < kEpiWarps; ++w) mbar_init(&bars->term_full[w], 1);
         bars->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -288,19 +348,13 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
-    // The launch before this one (programmatic dependency): everything above may overlap its end, everything
-    // below reads what it wrote.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) bars->skip = *reinterpret_cast<volatile uint32_t *>(error.device);
     tcgen05_fence_before();
     __syncthreads();
     if (kCtas == 2) cluster_sync_all();
     tcgen05_fence_after();
     const uint32_t tmem_base = bars->tmem_base;
-    // an earlier kernel gave up a wait: its output is half written, so nothing is computed from it.  Both
-    // CTAs of a pair read the same word after that kernel's end, so they agree.
-    if (bars->skip != 0u) n_tiles = 0;
+    if (bars->skip != 0u) n_tiles = 0;  // an earlier call gave up a wait
 
     if (warp == 0) {
         // ---- TMA producer: lane 0 fetches A and announces the bytes, lane 1 fetches B ----
@@ -314,7 +368,13 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 next = fetch_tile(launch, active, t + n_groups);
                 if (ti.skipped) continue;
                 const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * 128;
-                const int plane_rows = lane == 0 ? ti.p->plane_rows_a : ti.p->plane_rows_b;
+                const int plane_rows = ti.p->plane_rows;
+                if (!__all_sync(0x3u, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device, abort_flag,
+                                                  wait_limit))) {
+                    ok = false;
+                    break;
+                }
+                asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what other SMs stored
                 for (int kb = 0; kb < ti.k_blocks; ++kb) {
                     if (!__all_sync(0x3u, mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, wait_limit))) {
                         ok = false;
@@ -410,7 +470,9 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         // ---- epilogue: warp w reads TMEM lane quarter w % 4 and half of the columns ----
         constexpr int kCols = C::BN / 2;
         const int quarter = warp & 3, col_half = (warp - kFirstEpiWarp) >> 2;
-        const uint32_t my_stage = smem_u32(epi_stage) + (uint32_t)((warp - kFirstEpiWarp) * kStageWarpBytes);
+        uint8_t *const my_buffers = epi_stage + (size_t)(warp - kFirstEpiWarp) * kEpiWarpBytes;
+        uint64_t *const term_full = &bars->term_full[warp - kFirstEpiWarp];
+        uint32_t term_phase = 0;
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -427,77 +489,86 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             }
             const int row0 = ti.m0 + (int)cta_rank * BM + quarter * 32;
             const int col0 = ti.n0 + col_half * kCols;
-            // extents are multiples of 128: a warp's piece is all in or all out
+            // extents are multiples of 128: a warp's share is all in or all out
             const bool inside = row0 < p->M && col0 < p->N;
-            float sum[kPlanes == 2 ? kCols : 1];
-            if (kPlanes == 2) {  // the polynomial's other terms first: their loads overlap the first products
-                const int64_t at = (int64_t)(row0 + lane) * p->ld + col0;
-#pragma unroll
-                for (int j = 0; j < kCols; ++j) sum[kPlanes == 2 ? j : 0] = 0.0f;
-                if (inside && p->E != nullptr) {
-#pragma unroll
-                    for (int cc = 0; cc < kCols / 32; ++cc) {
-                        add_term<2>(sum, kPlanes == 2 ? cc * 32 : 0, p->e * mult, p->E + at + cc * 32, p->plane_d);
-                        asm volatile("" ::: "memory");  // no more than a piece's loads in registers at once
-                    }
-                }
-                if (inside && p->F != nullptr) {
-#pragma unroll
-                    for (int cc = 0; cc < kCols / 32; ++cc) {
-                        add_term<2>(sum, kPlanes == 2 ? cc * 32 : 0, p->f * mult, p->F + at + cc * 32, p->plane_d);
-                        asm volatile("" ::: "memory");
-                    }
-                }
-            }
-            const float cg = p->g * mult;
-            for (int k0 = 0; k0 < ti.k_blocks && ok; k0 += C::kChunkBlocks) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[acc], acc_phase, abort_flag, wait_limit))) {
+            Drain<kPlanes, kCols> drain{p, my_buffers, term_full, term_phase, row0, col0, lane, p->n_terms * kPlanes, ti.mirror};
+            if (inside && drain.per_piece > 0) {  // the first term: its matrix must be stored
+                if (!__all_sync(0xffffffffu, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device,
+                                                         abort_flag, wait_limit))) {
                     ok = false;
                     break;
                 }
-                tcgen05_fence_after();
-                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * C::BN + col_half * kCols);
-                if (kPlanes == 1) {
-                    if (inside) drain<kPlanes, kCols>(taddr, p, row0, col0, ti.mirror, mult, lane, my_stage);
-                } else {
-#pragma unroll
-                    for (int cc = 0; cc < kCols / 32; ++cc) {
-                        uint32_t v[32];
-                        tmem_ld_32x32_sync(taddr + (uint32_t)(cc * 32), v);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            sum[kPlanes == 2 ? cc * 32 + j : 0] =
-                                fmaf(cg, __uint_as_float(v[j]), sum[kPlanes == 2 ? cc * 32 + j : 0]);
-                    }
-                    if (k0 + C::kChunkBlocks >= ti.k_blocks && inside) {
-                        // finished: back into this warp's part of the accumulator, drained from there piece by piece
-#pragma unroll
-                        for (int cc = 0; cc < kCols / 32; ++cc) {
-                            uint32_t v[32];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[kPlanes == 2 ? cc * 32 + j : 0]);
-                            tmem_st_32x32(taddr + (uint32_t)(cc * 32), v);
-                        }
-                        tmem_st_wait();
-                        drain<kPlanes, kCols>(taddr, p, row0, col0, ti.mirror, mult, lane, my_stage);
-                    }
-                }
+                asm volatile("fence.proxy.async;" ::: "memory");
+                drain.fetch(0);
+            }
+            auto drained = [&](int buffer) {
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (kCtas == 2) mbar_remote_arrive(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
-                    else mbar_arrive(&bars->tmem_empty[acc]);
+                    if (kCtas == 2) mbar_remote_arrive(map_to_cta(smem_u32(&bars->tmem_empty[buffer]), 0));
+                    else mbar_arrive(&bars->tmem_empty[buffer]);
                 }
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
+            };
+            const uint32_t my_tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(col_half * kCols);
+            auto wait_acc = [&] {
+                const bool full = __all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[acc], acc_phase, abort_flag, wait_limit));
+                tcgen05_fence_after();
+                return full;
+            };
+            if (kPlanes == 2) {
+                float sum[kCols];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
+                const int chunks = (ti.k_blocks + C::kChunkBlocks - 1) / C::kChunkBlocks;
+                for (int c = 0; c + 1 < chunks && ok; ++c) {
+                    ok = wait_acc();
+                    if (!ok) break;
+#pragma unroll
+                    for (int cc = 0; cc < kCols / 32; ++cc) {
+                        uint32_t v[32];
+                        tmem_ld_32x32_sync(my_tmem + (uint32_t)(acc * C::BN + cc * 32), v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[cc * 32 + j] += __uint_as_float(v[j]);
+                    }
+                    drained(acc);
+                    acc ^= 1;
+                    acc_phase ^= acc == 0 ? 1u : 0u;
                 }
+                if (ok) ok = wait_acc();
+                if (!ok) break;
+                // the last piece joins, and the sum goes back into this warp's part of the accumulator, to be
+                // drained from there: the sum and the drain do not fit the registers together
+#pragma unroll
+                for (int cc = 0; cc < kCols / 32; ++cc) {
+                    uint32_t v[32];
+                    tmem_ld_32x32_sync(my_tmem + (uint32_t)(acc * C::BN + cc * 32), v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[cc * 32 + j] + __uint_as_float(v[j]));
+                    tmem_st_32x32(my_tmem + (uint32_t)(acc * C::BN + cc * 32), v);
+                }
+                tmem_st_wait();
+            } else {
+                ok = wait_acc();
+                if (!ok) break;
+            }
+            if (inside) ok = drain.run(my_tmem + (uint32_t)(acc * C::BN), mult, abort_flag, wait_limit, [&] { drained(acc); });
+            else drained(acc);
+            acc ^= 1;
+            acc_phase ^= acc == 0 ? 1u : 0u;
+            if (ok) {  // this warp's part of D is in memory, for TMA loads of other SMs
+                if (lane == 0) {
+                    bulk_wait_all();
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(launch.stored + ti.matrix) : "memory");
+                }
+                __syncwarp();
             }
         }
         if (!ok && lane == 0) {
             bars->abort = 1;
             report(error, 3u);
         }
+        if (lane == 0) bulk_wait_all();  // no store reads shared memory after this
         __syncwarp();
     }
 
@@ -508,6 +579,9 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         for (int s = 0; s < C::kStages; ++s)
             for (uint32_t i = 0; i < 4096u; ++i)
                 if (mbar_try_wait(&bars->full[s], 0) || mbar_try_wait(&bars->full[s], 1)) break;
+        for (int w = 0; w < kEpiWarps; ++w)
+            for (uint32_t i = 0; i < 4096u; ++i)
+                if (mbar_try_wait(&bars->term_full[w], 0) || mbar_try_wait(&bars->term_full[w], 1)) break;
     }
     __syncthreads();
     if (kCtas == 2) cluster_sync_all();
@@ -539,16 +613,32 @@ int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, i
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeCooperative;  // all CTAs resident at once, or the launch is refused
+    attr[0].val.cooperative = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = kCtas;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = kCtas == 2 ? 2 : 1;
-    // groups never wait for one another, so a grid larger than the device holds would still be right
-    const int groups = std::min(sm_count / kCtas, l.n_tiles);
+    int resident = sm_count;
+    if (kCtas == 2) {
+        static int max_clusters = 0;  // a device function of the kernel: pairs that fit at once
+        if (max_clusters == 0) {
+            cfg.gridDim = dim3((unsigned)(sm_count / 2 * 2));
+            cudaLaunchAttribute only[1] = {attr[1]};
+            cfg.attrs = only;
+            cfg.numAttrs = 1;
+            int count = 0;
+            VB_CUDA(cudaOccupancyMaxActiveClusters(&count, ns_product_kernel<kCtas, kPlanes>, &cfg));
+            if (count < 1) return fail(VB_ERR_CUDA, "the device cannot hold a 2-CTA cluster of the product kernel");
+            max_clusters = count;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+        }
+        resident = std::min(sm_count, 2 * max_clusters);
+    }
+    const int groups = std::min(resident / kCtas, l.n_tiles);
     cfg.gridDim = dim3((unsigned)(groups * kCtas));
     VB_CUDA(cudaLaunchKernelEx(&cfg, ns_product_kernel<kCtas, kPlanes>, l, d_active, error, wait_limit, withhold ? 1 : 0));
     return VB_OK;
@@ -558,9 +648,7 @@ int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, i
 
 void ns_tile_extent(int shape, int *bm, int *bn) { *bm = *bn = shape == NS_TILE_PAIR_256 ? 256 : 128; }
 
-// Tensor map over a row-major f16 matrix [outer][inner], 128-byte swizzle: 64 x 128 boxes, or (mn_major)
-// 64 x 64 x 2 boxes of the 3-D view [inner / 64][outer][64].
-int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, bool mn_major)
+int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int kind)
 {
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
@@ -571,23 +659,14 @@ int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer
             fn = reinterpret_cast<EncodeTiledFn>(sym);
     }
     if (!fn) return fail(VB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    CUresult r;
+    const bool view = kind == NS_MAP_MN;
     cuuint32_t estr[3] = {1, 1, 1};
-    if (mn_major) {
-        cuuint64_t dims[3] = {64, (cuuint64_t)outer, (cuuint64_t)(inner / 64)};
-        cuuint64_t strides[2] = {(cuuint64_t)inner * 2, 128};
-        cuuint32_t box[3] = {64, 64, 2};
-        r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    } else {
-        cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-        cuuint64_t strides[1] = {(cuuint64_t)inner * 2};
-        cuuint32_t box[2] = {64, 128};
-        r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    }
+    cuuint64_t dims[3] = {view ? 64 : (cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)(inner / 64)};
+    cuuint64_t strides[2] = {(cuuint64_t)inner * 2, 128};
+    cuuint32_t box[3] = {kind == NS_MAP_MIRROR ? 32u : 64u, kind == NS_MAP_ROWS ? 128u : kind == NS_MAP_PIECE ? 32u : 64u, 2};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, view ? 3 : 2, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, kind == NS_MAP_MIRROR ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(VB_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
     return VB_OK;
 }
@@ -596,7 +675,6 @@ int launch_ns_products(const NsLaunch &l, int shape, int planes, const uint32_t 
                        int sm_count, cudaStream_t stream, uint32_t wait_limit, bool withhold)
 {
     if (l.n_tiles <= 0) return VB_OK;
-    if (wait_limit == 0) wait_limit = kDefaultWaitLimit;
     if (shape == NS_TILE_PAIR_256)
         return planes == 2 ? launch_variant<2, 2>(l, d_active, error, sm_count, stream, wait_limit, withhold)
                            : launch_variant<2, 1>(l, d_active, error, sm_count, stream, wait_limit, withhold);
