@@ -95,7 +95,7 @@ static_assert(smem_bytes<2, 1>() <= 232448 && smem_bytes<1, 2>() <= 232448, "a C
 
 // 128 rows x 64 k of one plane: one box of a [rows][k] matrix, or one 64 x 64 x 2 box of [k][rows].
 template <int kCtas>
-__device__ __forceinline__ void load_rows(uint8_t *dst, const CUtensorMap *map, bool mn_major, int row0, int k0,
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, bool mn_major, int row0, int k0,
                                           int plane_rows, uint32_t bar)
 {
     if (mn_major) tma_load_3d<kCtas>(dst, map, 0, k0 + plane_rows, row0 >> 6, bar);
@@ -357,11 +357,14 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     if (bars->skip != 0u) n_tiles = 0;  // an earlier call gave up a wait
 
     if (warp == 0) {
-        // ---- TMA producer: lane 0 fetches A and announces the bytes, lane 1 fetches B ----
-        if (lane < 2) {
+        // ---- TMA producer ----
+        if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
+            const uint32_t slots = smem_u32(smem), empty0 = smem_u32(&bars->empty[0]);
+            // the leader announces the bytes of both CTAs; the peer's may land before that, the phase cannot end before it
+            const uint32_t full0 = kCtas == 2 ? map_to_cta(smem_u32(&bars->full[0]), 0) : smem_u32(&bars->full[0]);
             Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
             for (int t = group_id; t < n_tiles && ok; t += n_groups) {
                 const Tile ti = next;
@@ -369,33 +372,27 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 if (ti.skipped) continue;
                 const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * 128;
                 const int plane_rows = ti.p->plane_rows;
-                if (!__all_sync(0x3u, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device, abort_flag,
-                                                  wait_limit))) {
+                const CUtensorMap *map_a = &ti.p->map_a, *map_b = &ti.p->map_b;
+                if (!wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device, abort_flag, wait_limit)) {
                     ok = false;
                     break;
                 }
                 asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what other SMs stored
+#pragma unroll 1
                 for (int kb = 0; kb < ti.k_blocks; ++kb) {
-                    if (!__all_sync(0x3u, mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, wait_limit))) {
+                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, wait_limit)) {
                         ok = false;
                         break;
                     }
-                    uint8_t *slot = smem + (size_t)stage * C::kStageBytes;
-                    const uint32_t full_bar =
-                        kCtas == 2 ? map_to_cta(smem_u32(&bars->full[stage]), 0) : smem_u32(&bars->full[stage]);
-                    if (withhold) {
-                        // nothing is announced or staged: the bounded waits run out
-                    } else if (lane == 0) {
+                    if (!withhold) {  // withheld: nothing is announced or staged, the bounded waits run out
+                        const uint32_t slot = slots + (uint32_t)stage * C::kStageBytes, full = full0 + 8 * stage;
                         if (cta_rank == 0) mbar_expect_tx(&bars->full[stage], kCtas * C::kStageBytes);
 #pragma unroll
-                        for (int pl = 0; pl < kPlanes; ++pl)
-                            load_rows<kCtas>(slot + pl * C::kPlaneBytes, &ti.p->map_a, false, a_row0, kb * BK,
-                                             pl * plane_rows, full_bar);
-                    } else {
-#pragma unroll
-                        for (int pl = 0; pl < kPlanes; ++pl)
-                            load_rows<kCtas>(slot + pl * C::kPlaneBytes + kRows128Bytes, &ti.p->map_b, ti.b_mn, b_row0,
-                                             kb * BK, pl * plane_rows, full_bar);
+                        for (int pl = 0; pl < kPlanes; ++pl) {
+                            load_rows<kCtas>(slot + pl * C::kPlaneBytes, map_a, false, a_row0, kb * BK, pl * plane_rows, full);
+                            load_rows<kCtas>(slot + pl * C::kPlaneBytes + kRows128Bytes, map_b, ti.b_mn, b_row0, kb * BK,
+                                             pl * plane_rows, full);
+                        }
                     }
                     if (++stage == C::kStages) {
                         stage = 0;
@@ -415,12 +412,19 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
+            // One thread feeds the tensor core: what it computes per MMA must stay small, so descriptors are made
+            // once (for slot 0) and moved by adding 16-byte units to their address field.
+            const uint64_t desc_k = operand_desc(smem_u32(smem), false, 0), desc_mn = operand_desc(smem_u32(smem), true, 0);
+            const uint32_t full0 = smem_u32(&bars->full[0]);
             Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
             for (int t = group_id; t < n_tiles && ok; t += n_groups) {
                 const Tile ti = next;
                 next = fetch_tile(launch, active, t + n_groups);
                 if (ti.skipped) continue;
                 const uint32_t idesc = make_idesc(ti.b_mn, BM * kCtas, C::BN);
+                // B's descriptor differs by its major-ness in the fields above the address and in the step of a k slice
+                const uint64_t desc_b0 = ti.b_mn ? desc_mn : desc_k;
+                const uint32_t step_b = ti.b_mn ? 2048 >> 4 : 32 >> 4;
                 for (int k0 = 0; k0 < ti.k_blocks && ok; k0 += C::kChunkBlocks) {
                     const int k1 = min(k0 + C::kChunkBlocks, ti.k_blocks);
                     if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, wait_limit)) {
@@ -429,22 +433,24 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                     }
                     tcgen05_fence_after();
                     const uint32_t tmem_d = tmem_base + (uint32_t)(acc * C::BN);
+#pragma unroll 1
                     for (int kb = k0; kb < k1; ++kb) {
-                        if (!mbar_wait(&bars->full[stage], phase, abort_flag, wait_limit)) {
+                        if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, wait_limit)) {
                             ok = false;
                             break;
                         }
                         tcgen05_fence_after();
-                        const uint32_t base = smem_u32(smem + (size_t)stage * C::kStageBytes);
+                        const uint32_t slot = (uint32_t)stage * (C::kStageBytes >> 4);
                         // two planes: three products, smallest first; the dropped low x low is below 2^-22
 #pragma unroll
                         for (int term = 0; term < (kPlanes == 2 ? 3 : 1); ++term) {
-                            const uint32_t sa = base + (kPlanes == 2 && term == 1 ? C::kPlaneBytes : 0);
-                            const uint32_t sb = base + kRows128Bytes + (kPlanes == 2 && term == 0 ? C::kPlaneBytes : 0);
+                            const uint64_t da = desc_k + slot + (kPlanes == 2 && term == 1 ? C::kPlaneBytes >> 4 : 0);
+                            const uint64_t db = desc_b0 + slot + (kRows128Bytes >> 4) +
+                                                (kPlanes == 2 && term == 0 ? C::kPlaneBytes >> 4 : 0);
 #pragma unroll
                             for (int kk = 0; kk < BK / UMMA_K; ++kk)
-                                tcgen05_mma_bf16<kCtas>(tmem_d, operand_desc(sa, false, kk), operand_desc(sb, ti.b_mn, kk),
-                                                        idesc, (kb > k0 || term > 0 || kk > 0) ? 1u : 0u);
+                                tcgen05_mma_bf16<kCtas>(tmem_d, da + kk * (32 >> 4), db + kk * step_b, idesc,
+                                                        (kb > k0 || term > 0 || kk > 0) ? 1u : 0u);
                         }
                         tcgen05_commit<kCtas>(&bars->empty[stage]);
                         if (++stage == C::kStages) {

@@ -27,7 +27,7 @@ __device__ __forceinline__ void mbar_remote_arrive(uint32_t cluster_addr)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)  // shared-memory address
 {
     uint32_t ok;
     asm volatile(
@@ -35,13 +35,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
+        : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) { return mbar_try_wait(smem_u32(bar), parity); }
 // Bounded wait.  Returns false if the barrier did not flip in time or another role aborted.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag,
-                                          uint32_t wait_limit)
+template <typename Bar>
+__device__ __forceinline__ bool mbar_wait(Bar bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t wait_limit)
 {
     for (uint32_t i = 0; i < wait_limit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -68,39 +69,49 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t local, uint32_t rank)
     return r;
 }
 
-// TMA loads into this CTA's shared memory.  `bar` is a shared::cluster address: this CTA's own
+// TMA loads into this CTA's shared memory (address, or a pointer to it).  `bar` is a shared::cluster address: this CTA's own
 // barrier, or (kCtas == 2, .cta_group::2) the leader's.  Every CTA fetches its own rows.
 template <int kCtas>
-__device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *map, int c0, int c1, uint32_t bar)
+__device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap *map, int c0, int c1, uint32_t bar)
 {
     if (kCtas == 2)
         asm volatile(
             "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
             "[%0], [%1, {%2, %3}], [%4];"
-            ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+            ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
             : "memory");
     else
         asm volatile(
             "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-            ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+            ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
             : "memory");
 }
 template <int kCtas>
-__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, int c0, int c1, int c2,
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap *map, int c0, int c1, int c2,
                                             uint32_t bar)
 {
     if (kCtas == 2)
         asm volatile(
             "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
             "[%0], [%1, {%2, %3, %4}], [%5];"
-            ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+            ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
             : "memory");
     else
         asm volatile(
             "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
             "[%0], [%1, {%2, %3, %4}], [%5];"
-            ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+            ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
             : "memory");
+}
+template <int kCtas>
+__device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *map, int c0, int c1, uint32_t bar)
+{
+    tma_load_2d<kCtas>(smem_u32(smem_dst), map, c0, c1, bar);
+}
+template <int kCtas>
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar)
+{
+    tma_load_3d<kCtas>(smem_u32(smem_dst), map, c0, c1, c2, bar);
 }
 template <int kCtas>
 __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *map, int c0, int c1, int c2, int c3,
