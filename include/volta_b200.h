@@ -541,15 +541,14 @@ int vb_multi_tensor_step_static(vb_engine *engine, const vb_optimizer_step_param
 typedef struct vb_ns_plan vb_ns_plan;
 typedef struct vb_ns_matrices vb_ns_matrices;
 
-/* Pure host planning, no CUDA call: the products that a plan runs for one matrix (VB_NS_F16 and
- * VB_NS_F32_TC alike), for hosts and tests that want to check or cost the schedule.  Buffers 0
+/* Pure host planning, no CUDA call: the products that a plan of ns_mode runs for one matrix, for hosts and tests that want to check or cost the schedule.  Buffers 0
  * and 1 hold the working matrix X (n x m), 2 .. 6 short-side matrices; product k computes
  *     D = e E + f F + g A B'      (B' = B for an update of X, else B^T), times s^scale_power
  * where X_0 = s * (buffer 0).  ints: 9 per product {stage, A, B, E, F, D, scale_power, update, gram},
  * -1 for an absent term; products of one stage are independent.  doubles: 3 per product {e, f, g}.
  * The result is the last product's D times *final_scale.  Arrays may be NULL to query *n_products. */
-int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *coefficients, int64_t capacity,
-                          int64_t *n_products, int32_t *ints, double *doubles, double *final_scale);
+int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *coefficients, int ns_mode,
+                          int64_t capacity, int64_t *n_products, int32_t *ints, double *doubles, double *final_scale);
 
 int vb_ns_plan_create(vb_engine *engine, int64_t n_matrices, const int64_t *rows, const int64_t *cols, int n_steps,
                       const float *coefficients, float eps, int ns_mode, vb_ns_plan **out);

@@ -29,9 +29,9 @@ MIXED = [(8.0, -22.0, 16.0), (4.0, -2.9, 0.55), (1.5, -0.5, 0.0), (3.3, -2.4, 0.
 
 # ---- host only ---------------------------------------------------------------------------------
 
-def _products(rows, cols, coefficients):
+def _products(rows, cols, coefficients, mode=3):
     from volta_b200 import plan_newton_schulz
-    return plan_newton_schulz(rows, cols, coefficients)
+    return plan_newton_schulz(rows, cols, coefficients, mode)
 
 
 def _run_schedule(products, x0, coefficients):
@@ -61,14 +61,15 @@ def _run_schedule(products, x0, coefficients):
     return buffers
 
 
-@pytest.mark.parametrize("shape", [(24, 24), (16, 80), (80, 16), (1, 7), (1, 1), (33, 48)])
+@pytest.mark.parametrize("mode", [3, 2], ids=["f16", "f32"])
+@pytest.mark.parametrize("shape", [(24, 24), (16, 80), (80, 16), (1, 7), (1, 1), (33, 48), (70, 70), (300, 72)])
 @pytest.mark.parametrize("coefficients", [QUINTIC, CUBIC, MIXED, QUINTIC[:1], CUBIC[:2], [(1.0, 0.0, 0.0)],
                                           [(2.0, -1.5, 0.5)] * 12])
-def test_planned_products_are_the_iteration(shape, coefficients):
+def test_planned_products_are_the_iteration(shape, coefficients, mode):
     rng = np.random.default_rng(3)
     u = rng.standard_normal(shape)
     x = u.T if shape[0] > shape[1] else u
-    products, final_scale = _products(*shape, coefficients)
+    products, final_scale = _products(*shape, coefficients, mode)
     out = _run_schedule(products, x, coefficients)
     want = x / np.linalg.norm(x)
     for a, b, c in coefficients:
@@ -81,12 +82,14 @@ def test_planned_products_are_the_iteration(shape, coefficients):
 
 def test_groups_follow_the_amplification_limits():
     """Long matrices: the quintic runs in groups of 3 and 2 (of 2, 2 and 1 where the short side is small), square
-    ones step by step, the cubic as one."""
-    grams = lambda shape, co: [p["stage"] for p in _products(*shape, co)[0] if p["gram"]]  # noqa: E731
+    ones step by step, the cubic as one; short sides of at most 64 as one group in f16, in pairs to f32 accuracy."""
+    grams = lambda shape, co, mode=3: [p["stage"] for p in _products(*shape, co, mode)[0] if p["gram"]]  # noqa: E731
     assert len(grams((1024, 256), QUINTIC)) == 2
-    assert len(grams((64, 256), QUINTIC)) == 3
-    assert len(grams((64, 64), QUINTIC)) == 5
-    assert len(grams((256, 64), CUBIC)) == 1
+    assert len(grams((100, 256), QUINTIC)) == 3
+    assert len(grams((100, 100), QUINTIC)) == 5
+    assert len(grams((256, 100), CUBIC)) == 1
+    assert len(grams((64, 256), QUINTIC)) == 1
+    assert len(grams((64, 256), QUINTIC, 2)) == 3
 
 
 def test_plan_refuses_without_a_device_call():

@@ -137,7 +137,7 @@ SIGNATURES = {
     "vb_muon_last_ns_flops": [_vp, C.POINTER(C.c_double)],
     "vb_multi_tensor_step": [_vp, C.POINTER(StepParams), _i64, _i64p, _vpp, _vpp, _vpp, _vpp],
     "vb_multi_tensor_step_static": [_vp, C.POINTER(StepParams), _i64, _i64p, _vpp, _vpp, _vpp, _vpp],
-    "vb_plan_newton_schulz": [_i64, _i64, C.c_int, _f32p, _i64, _i64p, C.POINTER(C.c_int32), C.POINTER(C.c_double),
+    "vb_plan_newton_schulz": [_i64, _i64, C.c_int, _f32p, C.c_int, _i64, _i64p, C.POINTER(C.c_int32), C.POINTER(C.c_double),
                               C.POINTER(C.c_double)],
     "vb_ns_plan_create": [_vp, _i64, _i64p, _i64p, C.c_int, _f32p, C.c_float, C.c_int, _vpp],
     "vb_ns_plan_destroy": [_vp],

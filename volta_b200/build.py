@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libvolta_b200.so")
 
-SOURCES = ["api.cu", "multi_tensor.cu", "muon.cu", "ns_gemm_f32.cu", "ns_gemm_tc.cu", "ns_plan.cu", "ns_gather.cu", "ns_products.cu",
+SOURCES = ["api.cu", "multi_tensor.cu", "muon.cu", "ns_gemm_f32.cu", "ns_gemm_tc.cu", "ns_plan.cu", "ns_gather.cu", "ns_products.cu", "ns_small.cu",
            "exchange_fence.cu", "comm.cpp"]
 
 # No --use_fast_math: the Adam/SGD kernels promise bit parity with IEEE f32 arithmetic,

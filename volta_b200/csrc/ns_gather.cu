@@ -16,9 +16,7 @@
 // A tile is 64 x 128 of the working matrix (short side x long side).  Where an array's contiguous
 // direction is the tile's other one, the tile is turned in shared memory, so global accesses run
 // along memory for row-major and transposed arrays alike (any other strides: along j, element by element).
-#include <cuda_bf16.h>
-
-#include "ns_plan.h"
+#include "ns_elementwise.h"
 
 namespace vb {
 
@@ -26,62 +24,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPitch = kNsTileJ + 1;
-
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-template <> __device__ __forceinline__ float from_f32(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-
-// 8 elements along one direction (`step` apart in memory); the first `count` exist, the rest read as zero
-template <typename T>
-__device__ __forceinline__ void load8_as(const T *p, int64_t step, int count, bool vec, float (&v)[8])
-{
-    if (vec && count == 8) {
-        constexpr int kWords = (int)sizeof(T) * 8 / 16;
-        uint4 q[kWords];
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) q[w] = reinterpret_cast<const uint4 *>(p)[w];
-        const T *e = reinterpret_cast<const T *>(q);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = to_f32(e[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < count ? to_f32(p[k * step]) : 0.0f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store8_as(T *p, int64_t step, int count, bool vec, const float (&v)[8])
-{
-    if (vec && count == 8) {
-        constexpr int kWords = (int)sizeof(T) * 8 / 16;
-        uint4 q[kWords];
-        T *e = reinterpret_cast<T *>(q);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = from_f32<T>(v[k]);
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) reinterpret_cast<uint4 *>(p)[w] = q[w];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < count) p[k * step] = from_f32<T>(v[k]);
-    }
-}
-__device__ __forceinline__ void load8(int type, const void *base, int64_t at, int64_t step, int count, bool vec, float (&v)[8])
-{
-    if (type == VB_DTYPE_F32) load8_as(static_cast<const float *>(base) + at, step, count, vec, v);
-    else if (type == VB_DTYPE_BF16) load8_as(static_cast<const __nv_bfloat16 *>(base) + at, step, count, vec, v);
-    else load8_as(static_cast<const __half *>(base) + at, step, count, vec, v);
-}
-__device__ __forceinline__ void store8(int type, void *base, int64_t at, int64_t step, int count, bool vec, const float (&v)[8])
-{
-    if (type == VB_DTYPE_F32) store8_as(static_cast<float *>(base) + at, step, count, vec, v);
-    else if (type == VB_DTYPE_BF16) store8_as(static_cast<__nv_bfloat16 *>(base) + at, step, count, vec, v);
-    else store8_as(static_cast<__half *>(base) + at, step, count, vec, v);
-}
 
 // The tile's pass `k` (0..3) in one direction: this thread's 8 elements start at (i, j).
 struct Octet {
@@ -108,8 +50,6 @@ struct TileView {
         return left < 8 ? left : 8;
     }
 };
-// along i where that is the contiguous direction and j is not
-__device__ __forceinline__ bool walks_i(const NsArray &a) { return a.si == 1 && a.sj != 1; }
 __device__ __forceinline__ int64_t offset(const NsArray &a, const TileView &t, Octet o)
 {
     return (int64_t)(t.i0 + o.i) * a.si + (int64_t)(t.j0 + o.j) * a.sj;
@@ -145,16 +85,6 @@ __device__ __forceinline__ TileView tile_view(const NsMatrixDims &d, int tile)
 {
     const int per_row = d.mp / kNsTileJ, local = tile - d.tile0;
     return {(local / per_row) * kNsTileI, (local % per_row) * kNsTileJ, d.n, d.m};
-}
-
-// U of one octet in the velocity's direction: new velocity in v, U in u.
-__device__ __forceinline__ void momentum8(const NsElementwise &w, const float (&g)[8], float (&v)[8], float (&u)[8])
-{
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        v[e] = fmaf(w.momentum, v[e], g[e]);
-        u[e] = w.nesterov ? fmaf(w.momentum, v[e], g[e]) : v[e];
-    }
 }
 
 // The gradient goes through shared memory where its direction is not the velocity's.
@@ -321,7 +251,7 @@ ns_finish_kernel(const NsElementwise w, const __grid_constant__ NsBatchArgs b, c
     const TileView t = tile_view(d, index);
     const __half *x = w.x + d.final_off;
     const int64_t plane = (int64_t)d.np * d.mp;
-    constexpr int kOut = kStep ? 2 : 0;
+    constexpr int kOut = kStep ? 2 : 1;
     const NsArray &out = a.a[kOut];
     const bool vec = (a.direct >> kOut) & 1u;
     const bool oi = walks_i(out);

@@ -36,7 +36,6 @@ namespace {
 constexpr int kSquares = 5;  // short-side matrices alive at once: G, T, R, P and the one being written
 constexpr int kMaxSteps = 64;
 constexpr int64_t kMaxSide = 65536;
-constexpr double kFirstGroupGain = 150.0, kGroupGain = 17.0;
 constexpr uint32_t kDefaultWaitLimit = 1u << 22;  // polls, about a second
 constexpr double kDiverged = 1048576.0;
 // norm and gather of a batch follow each other; a batch's arrays should stay in the 126 MB L2 in between
@@ -70,7 +69,12 @@ int exponent_for(double bound)
     return std::min(e, 40);
 }
 
-std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, double first_gain)
+// How much a group may amplify the rounding of its Gram: the first one, and the others.  0: one step at a time.
+struct GroupLimits {
+    double first, later;
+};
+
+std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, const GroupLimits &limits)
 {
     std::vector<std::vector<int>> groups;
     std::vector<double> lam(4097);
@@ -78,7 +82,7 @@ std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, double
     double gain = 1.0;
     for (int k = 0; k < (int)steps.size(); ++k) {
         const Step &s = steps[(size_t)k];
-        const bool fits = !groups.empty() && gain <= (groups.size() == 1 ? first_gain : std::min(first_gain, kGroupGain));
+        const bool fits = !groups.empty() && gain <= (groups.size() == 1 ? limits.first : limits.later);
         if (!fits) {
             groups.emplace_back();
             gain = 1.0;
@@ -98,9 +102,9 @@ std::vector<std::vector<int>> make_groups(const std::vector<Step> &steps, double
 }
 
 // Returns false if the iterates leave the range that is sensible to hold.
-bool make_schedule(const std::vector<Step> &steps, double first_gain, Schedule *out)
+bool make_schedule(const std::vector<Step> &steps, const GroupLimits &limits, Schedule *out)
 {
-    const auto groups = make_groups(steps, first_gain);
+    const auto groups = make_groups(steps, limits);
     const int kSamples = 8192;
     std::vector<double> lam, sv;  // samples of the spectrum: of G, and the singular values of X
     for (int i = 0; i <= kSamples; ++i) lam.push_back((double)i / kSamples);
@@ -190,12 +194,39 @@ int read_steps(int n_steps, const float *coefficients, std::vector<Step> *steps)
     }
     return VB_OK;
 }
-// How much the first group of a matrix may amplify (0: one step at a time).
-double first_group_gain(int64_t rows, int64_t cols)
+// Matrices of ns_small.cu keep the short side in two planes whatever the mode: 2^-11 of the rounding, so that
+// much more amplification is allowed where f16 accuracy is asked for.
+GroupLimits group_limits(int64_t rows, int64_t cols, int planes, bool small)
+{
+    const double n = (double)std::min(rows, cols), m = (double)std::max(rows, cols);
+    if (small && planes == 1) return {5e4, 2e4};
+    if (small) return {75.0 * std::sqrt(n / 64.0), 17.0};
+    if (2.0 * m < 3.0 * n) return {0.0, 0.0};
+    return {150.0 * std::min(1.0, std::sqrt(n / 256.0)), 17.0};
+}
+bool is_small(int64_t rows, int64_t cols, int planes)
 {
     const int64_t n = std::min(rows, cols), m = std::max(rows, cols);
-    if (2 * m < 3 * n) return 0.0;
-    return kFirstGroupGain * std::min(1.0, std::sqrt((double)n / 256.0));
+    return n > 0 && n <= kNsSmallSide && m <= (int64_t)kNsSmallCluster * ns_small_columns(planes);
+}
+std::vector<NsSmallOp> small_program(const Schedule &s)
+{
+    std::vector<NsSmallOp> ops;
+    auto square = [](int buffer) { return (int8_t)(buffer >= BUF_SQUARE ? buffer - BUF_SQUARE : -1); };
+    for (const auto &stage : s.stages)
+        for (size_t k = 0; k < stage.size(); ++k) {
+            const Product &p = stage[k];
+            ops.push_back({square(p.A), square(p.B), square(p.E), square(p.F), square(p.D), (int8_t)(p.update ? 2 : p.gram ? 1 : 0),
+                           (int8_t)(k + 1 == stage.size()), (int8_t)p.scale_power, (float)p.e, (float)p.f, (float)p.g});
+        }
+    return ops;
+}
+
+int check_mode(int ns_mode)
+{
+    if (ns_mode == VB_NS_F16 || ns_mode == VB_NS_F32_TC) return VB_OK;
+    return fail(ns_mode == VB_NS_F32 || ns_mode == VB_NS_BF16 ? VB_ERR_UNSUPPORTED : VB_ERR_INVALID_ARG,
+                "a plan's ns_mode is VB_NS_F16 or VB_NS_F32_TC, not %d", ns_mode);
 }
 
 struct DeviceGuard {  // runs the call on the engine's device and leaves the caller's current one as it was
@@ -213,6 +244,15 @@ struct DeviceGuard {  // runs the call on the engine's device and leaves the cal
     }
 };
 
+// what ns_small.cu executes for one matrix: M = 128 with 64 rows in use, 64-column blocks, plane products
+double small_flops(const Schedule &s, int64_t m, int planes)
+{
+    double products = 0.0;
+    for (const auto &stage : s.stages)
+        for (const Product &p : stage)
+            products += p.gram ? (double)((m + 63) / 64) * (planes == 2 ? 3 : 1) : p.update ? (double)((m + 63) / 64) * (planes == 2 ? 3 : 2) : 3.0;
+    return products * 2.0 * 128 * 64 * 64;
+}
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 }  // namespace
@@ -247,6 +287,8 @@ struct vb_ns_plan {
         int32_t first, count, tile0, n_tiles;
     };
     std::vector<Batch> batches;
+    std::vector<int32_t> small_matrices;  // those that ns_small.cu runs, in its order
+    vb::NsSmall small{};
     vb::NsError error{};
     uint32_t *h_error = nullptr;
     bool withhold = false;
@@ -332,7 +374,12 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
     const int64_t n = p->n;
     std::vector<Schedule> schedules;       // the different ones among the matrices
     std::vector<std::vector<std::vector<int>>> groupings;
+    std::vector<std::vector<NsSmallOp>> programs;
     std::vector<size_t> kind((size_t)n);
+    std::vector<NsSmallMatrix> small;
+    std::vector<NsSmallOp> small_ops;
+    std::vector<int32_t> program_at;
+    int64_t small_m = 0;
     std::vector<int32_t> tile_matrix;
     std::vector<int64_t> square_off((size_t)n);
     int64_t x_total = 0, square_total = 0, tiles = 0, batch_elements = 0;
@@ -343,18 +390,36 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         d.n = (int32_t)std::min(p->rows[i], p->cols[i]);
         d.m = (int32_t)std::max(p->rows[i], p->cols[i]);
         if (d.n == 0) d.m = 0;
-        d.np = (int32_t)round_up(d.n, kNsPad);
-        d.mp = (int32_t)round_up(d.m, kNsPad);
-        const double gain = first_group_gain(d.n, d.m);
-        const auto groups = make_groups(steps, gain);
-        size_t which = 0;
-        while (which < groupings.size() && groupings[which] != groups) ++which;
-        if (which == groupings.size()) {
+        const auto limits = [&](bool as_small) { return group_limits(d.n, d.m, p->planes, as_small); };
+        auto find = [&](const GroupLimits &l, size_t *which) -> int {
+            const auto groups = make_groups(steps, l);
+            *which = 0;
+            while (*which < groupings.size() && groupings[*which] != groups) ++*which;
+            if (*which < groupings.size()) return VB_OK;
             groupings.push_back(groups);
             schedules.emplace_back();
-            if (!make_schedule(steps, gain, &schedules.back())) return fail(VB_ERR_INVALID_ARG, kDivergedText);
+            program_at.push_back(-1);
+            return make_schedule(steps, l, &schedules.back()) ? VB_OK : fail(VB_ERR_INVALID_ARG, kDivergedText);
+        };
+        size_t &which = kind[(size_t)i];
+        if (is_small(d.n, d.m, p->planes)) {
+            VB_TRY(find(limits(true), &which));
+            const auto ops = small_program(schedules[which]);
+            if (ops.size() <= kNsSmallOps) {
+                if (program_at[which] < 0) {
+                    program_at[which] = (int32_t)small_ops.size();
+                    small_ops.insert(small_ops.end(), ops.begin(), ops.end());
+                }
+                small.push_back({d.n, d.m, program_at[which], (int32_t)ops.size(), (float)schedules[which].final_scale});
+                p->small_matrices.push_back((int32_t)i);
+                small_m = std::max<int64_t>(small_m, d.m);
+                p->flops += small_flops(schedules[which], d.m, p->planes);
+                d.n = d.m = 0;  // nothing left for the other path
+            }
         }
-        kind[(size_t)i] = which;
+        if (d.n > 0 || p->small_matrices.empty() || p->small_matrices.back() != (int32_t)i) VB_TRY(find(limits(false), &which));
+        d.np = (int32_t)round_up(d.n, kNsPad);
+        d.mp = (int32_t)round_up(d.m, kNsPad);
         const Schedule &s = schedules[kind[(size_t)i]];
         d.x_off = x_total;
         d.final_off = s.final_buffer;  // buffer number for now
@@ -385,6 +450,16 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
     std::vector<NsProduct> problems;
     std::vector<NsTile> tile_list;
 
+    if (!small.empty()) {
+        // CTAs per matrix: as many as its columns need, more while the device has SMs and they have columns
+        const int64_t fit = ns_small_columns(p->planes), count = (int64_t)small.size();
+        int c = 1;
+        while (round_up((small_m + c - 1) / c, 64) > fit) c *= 2;
+        while (c < kNsSmallCluster && count * c * 2 <= p->eng->sm_count && small_m > 64 * c) c *= 2;
+        p->small.cluster = c;
+        p->small.columns = (int)round_up((small_m + c - 1) / c, 64);
+    }
+
     // The carving is done twice: for the size, then with the addresses (tensor maps need them).
     __half *x_base = nullptr, *square_base = nullptr;
     for (int round = 0; round < 2; ++round) {
@@ -402,6 +477,10 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         NsMatrixDims *d_dims = c.take<NsMatrixDims>((size_t)n);
         int32_t *d_tile_matrix = c.take<int32_t>(tile_matrix.size());
         p->ew.dims = d_dims;
+        NsSmallMatrix *d_small = c.take<NsSmallMatrix>(small.size());
+        NsSmallOp *d_small_ops = c.take<NsSmallOp>(small_ops.size());
+        p->small.matrices = d_small;
+        p->small.ops = d_small_ops;
         p->d_tile_matrix = d_tile_matrix;
         problems.clear();
         std::vector<size_t> stage_begin;  // of every stage's products in `problems`
@@ -468,7 +547,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
             int bm, bn;
             ns_tile_extent(p->shape, &bm, &bn);
-            double stage_flops = 0.0;
+            double stage_flops = 0.0;  // of the largest product
             for (size_t q = 0; q < problems.size(); ++q)
                 stage_flops = std::max(stage_flops, 2.0 * (double)problems[q].M * problems[q].N * problems[q].K * 3.0);
             // the default bound (about a second) plus two per 1e14 FLOPs of the largest product: a role may rightly
@@ -481,6 +560,10 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             p->workspace = c.used;
             VB_CUDA(cudaMalloc((void **)&p->d_base, std::max<size_t>(c.used, 1024)));
         } else {
+            if (!small.empty()) {
+                VB_CUDA(cudaMemcpyAsync(d_small, small.data(), small.size() * sizeof(NsSmallMatrix), cudaMemcpyHostToDevice, p->eng->stream));
+                VB_CUDA(cudaMemcpyAsync(d_small_ops, small_ops.data(), small_ops.size() * sizeof(NsSmallOp), cudaMemcpyHostToDevice, p->eng->stream));
+            }
             VB_CUDA(cudaMemsetAsync(p->error.device, 0, sizeof(uint32_t), p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_dims, p->dims.data(), (size_t)n * sizeof(NsMatrixDims), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tile_matrix, tile_matrix.data(), tile_matrix.size() * sizeof(int32_t), cudaMemcpyHostToDevice, p->eng->stream));
@@ -493,39 +576,51 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
     return VB_OK;
 }
 
-// What both operators share: per batch `fill` sets the arrays of one matrix.
+// What both operators share; `fill` sets the arrays of one matrix.
 template <typename Fill>
-int run_plan(vb_ns_plan *p, const NsElementwise &w, const NsElementwise &fin, bool step, Fill &&fill)
+int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
 {
     vb_engine *e = p->eng;
     NsBatchArgs &args = *p->args;
-    auto load = [&](const vb_ns_plan::Batch &b, bool finish) {
+    auto load = [&](const vb_ns_plan::Batch &b) {
         args.first = b.first;
         args.count = b.count;
         args.tile0 = b.tile0;
         args.n_tiles = b.n_tiles;
-        for (int32_t k = 0; k < b.count; ++k) fill(b.first + k, args.m[k], finish);
+        for (int32_t k = 0; k < b.count; ++k) fill(b.first + k, args.m[k]);
     };
+    const uint32_t wait_limit = p->wait_limit ? p->wait_limit : p->default_wait_limit;
     prof_begin(e, VB_PHASE_MUON_PRE);
     for (const auto &b : p->batches) {
-        load(b, false);
+        if (b.n_tiles == 0) continue;
+        load(b);
         VB_TRY(launch_ns_norm(w, args, p->d_tile_matrix, step, e->stream));
         VB_TRY(launch_ns_gather(w, args, p->d_tile_matrix, step, e->stream));
-        if (b.n_tiles > 0) e->launches += 2;
+        e->launches += 2;
     }
     prof_end(e, VB_PHASE_MUON_PRE);
     prof_begin(e, VB_PHASE_MUON_NS);
-    VB_TRY(launch_ns_products(p->products, p->shape, p->planes, w.active, p->error, e->sm_count, e->stream,
-                              p->wait_limit ? p->wait_limit : p->default_wait_limit, p->withhold));
-    p->withhold = false;
+    if (p->products.n_tiles > 0) {
+        VB_TRY(launch_ns_products(p->products, p->shape, p->planes, w.active, p->error, e->sm_count, e->stream, wait_limit, p->withhold));
+        e->launches += 1;
+        p->withhold = false;
+    }
+    for (size_t k0 = 0; k0 < p->small_matrices.size(); k0 += kNsBatch) {
+        args.first = (int32_t)k0;
+        args.count = (int32_t)std::min<size_t>(kNsBatch, p->small_matrices.size() - k0);
+        for (int32_t k = 0; k < args.count; ++k) fill(p->small_matrices[k0 + (size_t)k], args.m[k]);
+        VB_TRY(launch_ns_small(w, p->small, args, p->error, step, e->stream, wait_limit, p->withhold));
+        e->launches += 1;
+        p->withhold = false;
+    }
     p->wait_limit = 0;
-    if (p->products.n_tiles > 0) e->launches += 1;
     prof_end(e, VB_PHASE_MUON_NS);
     prof_begin(e, VB_PHASE_MUON_APPLY);
     for (const auto &b : p->batches) {
-        load(b, true);
-        VB_TRY(launch_ns_finish(fin, args, p->d_tile_matrix, step, e->stream));
-        if (b.n_tiles > 0) e->launches += 1;
+        if (b.n_tiles == 0) continue;
+        load(b);
+        VB_TRY(launch_ns_finish(w, args, p->d_tile_matrix, step, e->stream));
+        e->launches += 1;
     }
     prof_end(e, VB_PHASE_MUON_APPLY);
     return VB_OK;
@@ -573,8 +668,8 @@ using namespace vb;
 
 extern "C" {
 
-int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *coefficients, int64_t capacity,
-                          int64_t *n_products, int32_t *ints, double *doubles, double *final_scale)
+int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *coefficients, int ns_mode,
+                          int64_t capacity, int64_t *n_products, int32_t *ints, double *doubles, double *final_scale)
 {
     VB_NS_BEGIN
     if (!n_products) return fail(VB_ERR_INVALID_ARG, "n_products is null");
@@ -582,7 +677,9 @@ int vb_plan_newton_schulz(int64_t rows, int64_t cols, int n_steps, const float *
     std::vector<Step> steps;
     VB_TRY(read_steps(n_steps, coefficients, &steps));
     Schedule s;
-    if (!make_schedule(steps, first_group_gain(rows, cols), &s)) return fail(VB_ERR_INVALID_ARG, kDivergedText);
+    VB_TRY(check_mode(ns_mode));
+    const int planes = ns_mode == VB_NS_F32_TC ? 2 : 1;
+    if (!make_schedule(steps, group_limits(rows, cols, planes, is_small(rows, cols, planes)), &s)) return fail(VB_ERR_INVALID_ARG, kDivergedText);
     int64_t k = 0;
     for (size_t stage = 0; stage < s.stages.size(); ++stage)
         for (const Product &p : s.stages[stage]) {
@@ -611,9 +708,7 @@ int vb_ns_plan_create(vb_engine *e, int64_t n, const int64_t *rows, const int64_
     std::vector<Step> steps;
     VB_TRY(read_steps(n_steps, coefficients, &steps));
     if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(VB_ERR_INVALID_ARG, "eps must be finite and >= 0");
-    if (ns_mode != VB_NS_F16 && ns_mode != VB_NS_F32_TC)
-        return fail(ns_mode == VB_NS_F32 || ns_mode == VB_NS_BF16 ? VB_ERR_UNSUPPORTED : VB_ERR_INVALID_ARG,
-                    "a plan's ns_mode is VB_NS_F16 or VB_NS_F32_TC, not %d", ns_mode);
+    VB_TRY(check_mode(ns_mode));
     for (int64_t i = 0; i < n; ++i)
         if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxSide || cols[i] > kMaxSide)
             return fail(VB_ERR_INVALID_ARG, "matrix %lld is %lld x %lld: sides are 0 to %lld", (long long)i, (long long)rows[i], (long long)cols[i], (long long)kMaxSide);
@@ -753,12 +848,12 @@ int vb_orthogonalize(vb_ns_plan *p, const vb_ns_matrices *inputs, const vb_ns_ma
     w.planes = p->planes;
     w.eps = p->eps;
     w.types[0] = inputs->dtype;
-    NsElementwise fin = w;
-    fin.types[0] = outputs->dtype;
-    return run_plan(p, w, fin, false, [&](int64_t i, NsMatrixArg &a, bool finish) {
-        const vb_ns_matrices *source = finish ? outputs : inputs;
-        a.a[0] = source->arrays[(size_t)i];
-        a.direct = source->vec[(size_t)i];
+    w.types[1] = outputs->dtype;
+    return run_plan(p, w, false, [&](int64_t i, NsMatrixArg &a) {
+        const size_t k = (size_t)i;
+        a.a[0] = inputs->arrays[k];
+        a.a[1] = outputs->arrays[k];
+        a.direct = (uint32_t)inputs->vec[k] | (uint32_t)outputs->vec[k] << 1;
         a.live = 1;
         a.scale = 1.0f;
     });
@@ -790,7 +885,7 @@ int vb_muon_multi_tensor_step(vb_ns_plan *p, const vb_muon_step_params *hp, cons
     w.nesterov = hp->nesterov != 0;
     w.decay = (float)(1.0 - (double)hp->lr * (double)hp->weight_decay);
     w.rate = hp->lr;
-    return run_plan(p, w, w, true, [&](int64_t i, NsMatrixArg &a, bool) {
+    return run_plan(p, w, true, [&](int64_t i, NsMatrixArg &a) {
         const size_t k = (size_t)i;
         a.a[0] = grads->arrays[k];
         a.a[1] = velocities->arrays[k];

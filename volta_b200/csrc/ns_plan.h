@@ -84,7 +84,7 @@ struct NsArray {
 };
 constexpr int kNsBatch = 96;  // matrices of one element-wise launch (bounded by its parameter space)
 struct NsMatrixArg {
-    NsArray a[3];   // orthogonalize: input or output; step: gradient, velocity, parameter
+    NsArray a[3];   // orthogonalize: input, output; step: gradient, velocity, parameter
     float scale;    // step: s_i of the update
     uint32_t live;  // 0: no gradient, the matrix is left alone
     uint32_t direct; // bit k: array k has sj == 1 and rows on 16-byte boundaries
@@ -121,5 +121,32 @@ constexpr int kNsTileI = 64, kNsTileJ = 128;  // an element-wise tile of the wor
 int launch_ns_norm(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
 int launch_ns_gather(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
 int launch_ns_finish(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
+
+// ---- matrices with a short side of at most 64 (ns_small.cu) ----------------------------------
+constexpr int kNsSmallSide = 64;
+constexpr int kNsSmallOps = 128;     // longest program
+constexpr int kNsSmallSquares = 5;
+constexpr int kNsSmallCluster = 8;   // most CTAs of one matrix
+struct NsSmallOp {
+    int8_t A, B, E, F, D;   // short-side matrices (0 ..), -1: none; of a Gram D, of an update A only
+    int8_t kind;            // 0 product of two short-side matrices, 1 Gram, 2 update of X
+    int8_t stage_end;       // the next op depends on this one
+    int8_t scale_power;
+    float e, f, g;          // as in NsProduct
+};
+struct NsSmallMatrix {
+    int32_t n, m;
+    int32_t op0, n_ops;     // its program
+    float final_scale;
+};
+struct NsSmall {
+    const NsSmallMatrix *matrices;  // of a whole plan
+    const NsSmallOp *ops;
+    int cluster;                    // CTAs per matrix
+    int columns;                    // columns of X per CTA, a multiple of 64
+};
+int ns_small_columns(int planes);  // columns of X that fit one CTA
+int launch_ns_small(const NsElementwise &w, const NsSmall &s, const NsBatchArgs &b, NsError error, bool step, cudaStream_t stream,
+                    uint32_t wait_limit, bool withhold);
 
 }  // namespace vb

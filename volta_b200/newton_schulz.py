@@ -181,15 +181,15 @@ class NewtonSchulzPlan:
              (C.c_float * n)(*scales) if scales is not None else None)
 
 
-def plan_newton_schulz(rows: int, cols: int, coefficients: Sequence[Sequence[float]]):
+def plan_newton_schulz(rows: int, cols: int, coefficients: Sequence[Sequence[float]], ns_mode: int = VB_NS_F16):
     """The products a plan runs for one matrix (``vb_plan_newton_schulz``, no device needed): a list of
     dicts with the buffers and factors of ``D = e E + f F + g A B'``, and the factor of the last one's D."""
     flat = [float(v) for step in coefficients for v in step]
     co = (C.c_float * max(len(flat), 1))(*flat)
     n, scale = C.c_int64(), C.c_double()
-    call("vb_plan_newton_schulz", rows, cols, len(coefficients), co, 0, C.byref(n), None, None, C.byref(scale))
+    call("vb_plan_newton_schulz", rows, cols, len(coefficients), co, int(ns_mode), 0, C.byref(n), None, None, C.byref(scale))
     ints, doubles = (C.c_int32 * (9 * n.value))(), (C.c_double * (3 * n.value))()
-    call("vb_plan_newton_schulz", rows, cols, len(coefficients), co, n.value, C.byref(n), ints, doubles, C.byref(scale))
+    call("vb_plan_newton_schulz", rows, cols, len(coefficients), co, int(ns_mode), n.value, C.byref(n), ints, doubles, C.byref(scale))
     names = ("stage", "A", "B", "E", "F", "D", "scale_power", "update", "gram")
     return [dict(zip(names, ints[9 * k:9 * k + 9]), **dict(zip("efg", doubles[3 * k:3 * k + 3])))
             for k in range(n.value)], scale.value
