@@ -13,6 +13,8 @@
 // same bits and run the same short-side program, the planner's products (ns_plan.cu), with all of its matrices
 // in shared memory as two f16 planes.  With 22 bits on the short side the groups of steps can be long: in
 // VB_NS_F16 the five steps of a quintic are one group, so X is read twice and never rewritten.
+// What a stage costs (cycles, 64 x 288 to f32 accuracy): 12 MMAs 400, their completion 250, tensor memory to
+// shared memory 600, barriers 200.
 //
 // Shared memory: five squares of 16 KiB, the share of X, and 8 KiB that M = 128 operands run over into (rows
 // 64 .. 127 of A are whatever lies there; they only reach rows of the accumulator that nobody reads).
@@ -25,7 +27,8 @@ namespace vb {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kCols = 16;  // columns of a worker warp: 8 of the 16 warps reach TMEM lanes 0 .. 63
 constexpr int kSide = kNsSmallSide;
 constexpr int kBlockBytes = kSide * 128;          // 64 rows x 64 f16
 constexpr int kSquareBytes = 2 * kBlockBytes;     // two planes
@@ -54,15 +57,15 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b)
 }
 __device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 
-// f += c * (32 values of one row of a block, columns col .. col + 31, all planes)
+// f += c * (16 values of one row of a block, columns col .. col + 15, all planes)
 template <int kPlanes>
-__device__ __forceinline__ void add_row(float (&f)[32], float c, uint32_t block, int row, int col)
+__device__ __forceinline__ void add_row(float (&f)[kCols], float c, uint32_t block, int row, int col)
 {
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl) {
         const uint32_t at = block + (uint32_t)(pl * kBlockBytes + row * 128);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kCols / 8; ++q) {
             uint32_t v[4];
             ld_shared_128(at + (uint32_t)((((col >> 3) + q) ^ (row & 7)) << 4), v[0], v[1], v[2], v[3]);
 #pragma unroll
@@ -75,13 +78,13 @@ __device__ __forceinline__ void add_row(float (&f)[32], float c, uint32_t block,
     }
 }
 template <int kPlanes>
-__device__ __forceinline__ void put_row(float (&f)[32], uint32_t block, int row, int col)
+__device__ __forceinline__ void put_row(float (&f)[kCols], uint32_t block, int row, int col)
 {
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl) {
         const uint32_t at = block + (uint32_t)(pl * kBlockBytes + row * 128);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kCols / 8; ++q) {
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -98,13 +101,15 @@ __device__ __forceinline__ void put_row(float (&f)[32], uint32_t block, int row,
 }
 
 // A (128 x 64, rows from 64 on unused) times B (64 x 64) into 64 accumulator columns; operands are blocks of
-// kA and kB planes, the products of their planes smallest first.
+// kA and kB planes, the products of their planes smallest first.  `a` and `b` are descriptors of plane 0 (see
+// Descriptors): other planes and k slices are reached by adding to the address field.
 template <int kA, int kB>
-__device__ __forceinline__ void issue_product(uint32_t tmem, uint32_t a, uint32_t b, bool b_mn, bool accumulate)
+__device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_t b, bool b_mn, bool accumulate)
 {
     // f32 accumulator, f16 operands, A K-major, M = 128, N = 64
     const uint32_t idesc = (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(kSide >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-    bool first = !accumulate;
+    const uint32_t step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+    uint32_t keep = accumulate ? 1u : 0u;
 #pragma unroll
     for (int t = kA + kB - 2; t >= 0; --t) {  // plane of A + plane of B; low x low is dropped
         if (kA == 2 && kB == 2 && t == 2) continue;
@@ -114,15 +119,33 @@ __device__ __forceinline__ void issue_product(uint32_t tmem, uint32_t a, uint32_
             if (pb < 0 || pb >= kB) continue;
 #pragma unroll
             for (int kk = 0; kk < kSide / 16; ++kk) {
-                const uint32_t at_b = b + (uint32_t)(pb * kBlockBytes);
-                tcgen05_mma_bf16<1>(tmem, make_smem_desc(a + (uint32_t)(pa * kBlockBytes + kk * 32), 16, 1024),
-                                    b_mn ? make_smem_desc(at_b + kk * 2048, kBlockBytes, 1024)
-                                         : make_smem_desc(at_b + kk * 32, 16, 1024),
-                                    idesc, first ? 0u : 1u);
-                first = false;
+                tcgen05_mma_bf16<1>(tmem, a + (uint32_t)(pa * (kBlockBytes >> 4) + kk * (32 >> 4)),
+                                    b + (uint32_t)(pb * (kBlockBytes >> 4)) + kk * step_b, idesc, keep);
+                keep = 1u;
             }
         }
     }
+}
+// Descriptors of an operand block in shared memory: everything but the address is the same for all blocks.
+struct Descriptors {
+    uint64_t k_major, mn_major;  // of address 0
+    __device__ __forceinline__ Descriptors() : k_major(make_smem_desc(0, 16, 1024)), mn_major(make_smem_desc(0, kBlockBytes, 1024)) {}
+    __device__ __forceinline__ uint64_t rows(uint32_t addr) const { return k_major + (addr >> 4); }
+    __device__ __forceinline__ uint64_t columns(uint32_t addr) const { return mn_major + (addr >> 4); }
+};
+__device__ __forceinline__ void tmem_ld_16_sync(uint32_t taddr, float (&f)[kCols])
+{
+    uint32_t v[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(v[k]);
 }
 
 __device__ __forceinline__ double warp_sum(double v)
@@ -137,11 +160,16 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr)
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
     return v;
 }
+// volatile, so after the barrier before it; no memory clobber, so that several are in flight
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr)
 {
     float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
+}
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float4 v)
+{
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
 // The CTA's columns [j0, j1) of the caller's arrays, 8 elements at a time along the first array's direction.
@@ -162,31 +190,98 @@ struct Share {
         const int left = (j0 + j < m && i < n) ? (along_i ? n - i : m - j0 - j) : 0;
         count = left < 0 ? 0 : left < 8 ? left : 8;
     }
-    __device__ __forceinline__ void read(int type, const NsArray &a, bool vec, int i, int j, int count, float (&v)[8]) const
+    __device__ __forceinline__ int64_t offset(const NsArray &a, int i, int j) const { return (int64_t)i * a.si + (int64_t)(j0 + j) * a.sj; }
+    // a vector access runs along the array's own direction
+    __device__ __forceinline__ bool vec(const NsArray &a, bool aligned) const { return aligned && walks_i(a) == along_i; }
+    __device__ __forceinline__ void write(int type, const NsArray &a, bool aligned, int i, int j, int count, const float (&v)[8]) const
     {
-        // a vector access runs along the array's own direction
-        load8(type, a.ptr, (int64_t)i * a.si + (int64_t)(j0 + j) * a.sj, along_i ? a.si : a.sj, count,
-              vec && walks_i(a) == along_i, v);
-    }
-    __device__ __forceinline__ void write(int type, const NsArray &a, bool vec, int i, int j, int count, const float (&v)[8]) const
-    {
-        store8(type, a.ptr, (int64_t)i * a.si + (int64_t)(j0 + j) * a.sj, along_i ? a.si : a.sj, count,
-               vec && walks_i(a) == along_i, v);
+        store8(type, a.ptr, offset(a, i, j), along_i ? a.si : a.sj, count, vec(a, aligned), v);
     }
 };
 
-template <bool kStep>
-__device__ __forceinline__ void read_u(const NsElementwise &w, const NsMatrixArg &a, const Share &s, int i, int j, int count,
-                                       float (&v)[8], float (&u)[8])
-{
-    if (kStep) {
-        float g[8];
-        s.read(w.types[0], a.a[0], a.direct & 1u, i, j, count, g);
-        s.read(w.types[1], a.a[1], a.direct & 2u, i, j, count, v);
-        momentum8(w, g, v, u);
-    } else {
-        s.read(w.types[0], a.a[0], a.direct & 1u, i, j, count, u);
+// 8 elements as they lie in memory (whole and aligned octets) or as f32: loads first, conversions later, so that
+// a thread has several octets on their way.
+struct Raw {
+    uint4 q[2];
+    bool packed;
+    __device__ __forceinline__ void load(int type, const NsArray &a, const Share &s, bool aligned, int i, int j, int count)
+    {
+        packed = count == 8 && s.vec(a, aligned);
+        if (packed) {
+            const char *p = static_cast<const char *>(a.ptr) + s.offset(a, i, j) * (type == VB_DTYPE_F32 ? 4 : 2);
+            q[0] = *reinterpret_cast<const uint4 *>(p);
+            if (type == VB_DTYPE_F32) q[1] = reinterpret_cast<const uint4 *>(p)[1];
+        }
     }
+    __device__ __forceinline__ void get(int type, const NsArray &a, const Share &s, int i, int j, int count, float (&v)[8]) const
+    {
+        if (!packed) {
+            load8(type, a.ptr, s.offset(a, i, j), s.along_i ? a.si : a.sj, count, false, v);
+            return;
+        }
+        if (type == VB_DTYPE_F32) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                v[4 * k] = __uint_as_float(q[k].x), v[4 * k + 1] = __uint_as_float(q[k].y);
+                v[4 * k + 2] = __uint_as_float(q[k].z), v[4 * k + 3] = __uint_as_float(q[k].w);
+            }
+        } else {
+            const uint32_t h[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (type == VB_DTYPE_BF16) {
+                    v[2 * k] = __uint_as_float(h[k] << 16);
+                    v[2 * k + 1] = __uint_as_float(h[k] & 0xffff0000u);
+                } else {
+                    const float2 x = unpack_half(h[k]);
+                    v[2 * k] = x.x, v[2 * k + 1] = x.y;
+                }
+            }
+        }
+    }
+};
+
+// Calls fn(i, j, count, v, u) for this thread's octets of U (and, step, of the new velocity).
+constexpr int kInFlight = 4;
+template <bool kStep, typename Fn>
+__device__ __forceinline__ void for_u(const NsElementwise &w, const NsMatrixArg &a, const Share &s, Fn &&fn)
+{
+    for (int o0 = threadIdx.x; o0 < s.octets(); o0 += kThreads * kInFlight) {
+        Raw g[kInFlight], v[kStep ? kInFlight : 1];
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k) {
+            const int o = o0 + k * kThreads;
+            if (o >= s.octets()) break;
+            int i, j, count;
+            s.locate(o, i, j, count);
+            g[k].load(w.types[0], a.a[0], s, a.direct & 1u, i, j, count);
+            if (kStep) v[kStep ? k : 0].load(w.types[1], a.a[1], s, a.direct & 2u, i, j, count);
+        }
+#pragma unroll
+        for (int k = 0; k < kInFlight; ++k) {
+            const int o = o0 + k * kThreads;
+            if (o >= s.octets()) break;
+            int i, j, count;
+            s.locate(o, i, j, count);
+            float gg[8], vv[8], u[8];
+            g[k].get(w.types[0], a.a[0], s, i, j, count, gg);
+            if (kStep) {
+                v[kStep ? k : 0].get(w.types[1], a.a[1], s, i, j, count, vv);
+                momentum8(w, gg, vv, u);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[e] = gg[e];
+            }
+            fn(i, j, count, vv, u);
+        }
+    }
+}
+
+// 8 values of the planes of X in shared memory, along i (i a multiple of 8) or along j
+template <int kPlanes>
+__device__ __forceinline__ uint32_t x_address(uint32_t x_base, int i, int j)
+{
+    return x_base + (uint32_t)((j >> 6) * kPlanes * kBlockBytes + i * 128 + ((((j & 63) >> 3) ^ (i & 7)) << 4) + (j & 7) * 2);
 }
 
 __device__ __forceinline__ void report(const NsError &error)
@@ -215,7 +310,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     if (a.live == 0u) return;  // the whole cluster
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool worker = (warp & 3) < 2;  // TMEM lanes 0 .. 63
-    const int row = (warp & 3) * 32 + lane, col = (warp >> 2) * 32;
+    const int row = (warp & 3) * 32 + lane, col = (warp >> 2) * kCols;
 
     if (threadIdx.x == 0) {
         mbar_init(&sh.done, 1);
@@ -233,15 +328,10 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     // ---- the norm: every CTA of the cluster its columns, then all sums in rank order ----
     const Share s{d.n, d.m, rank * small.columns, small.columns, walks_i(a.a[kStep ? 1 : 0])};
     double sum = 0.0;
-#pragma unroll 4
-    for (int o = threadIdx.x; o < s.octets(); o += kThreads) {
-        int i, j, count;
-        s.locate(o, i, j, count);
-        float v[8], u[8];
-        read_u<kStep>(w, a, s, i, j, count, v, u);
+    for_u<kStep>(w, a, s, [&](int, int, int, const float (&)[8], const float (&u)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fma((double)u[e], (double)u[e], sum);
-    }
+    });
     sum = warp_sum(sum);
     if (lane == 0) sh.warp_sums[warp] = sum;
     tcgen05_fence_before();
@@ -265,14 +355,8 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     const float scale = isfinite(norm) ? (float)(ldexp(1.0, -shift) / (norm + (double)w.eps)) : nanf("");
 
     // ---- the share of X as f16 planes, blocks of 64 columns; step: the new velocity ----
-#pragma unroll 2
-    for (int o = threadIdx.x; o < s.octets(); o += kThreads) {
-        int i, j, count;
-        s.locate(o, i, j, count);
-        float v[8], u[8];
-        read_u<kStep>(w, a, s, i, j, count, v, u);
+    for_u<kStep>(w, a, s, [&](int i, int j, int count, const float (&v)[8], const float (&u)[8]) {
         if (kStep && !dead) s.write(w.types[1], a.a[1], a.direct & 2u, i, j, count, v);
-        const uint32_t block = x_base + (uint32_t)((j >> 6) * kPlanes * kBlockBytes);
         __half h[8], l[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -282,23 +366,24 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         }
         if (s.along_i) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {  // i is a multiple of 8: row & 7 == e
-                const uint32_t at = block + (uint32_t)((i + e) * 128 + ((((j & 63) >> 3) ^ e) << 4) + (j & 7) * 2);
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t at = x_address<kPlanes>(x_base, i + e, j);
                 asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(h[e])) : "memory");
                 if (kPlanes == 2) asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + kBlockBytes), "h"(__half_as_ushort(l[e])) : "memory");
             }
         } else {
-            const uint32_t at = block + (uint32_t)(i * 128 + ((((j & 63) >> 3) ^ (i & 7)) << 4));
+            const uint32_t at = x_address<kPlanes>(x_base, i, j);
             const uint4 qh = *reinterpret_cast<const uint4 *>(h), ql = *reinterpret_cast<const uint4 *>(l);
             st_shared_128(at, qh.x, qh.y, qh.z, qh.w);
             if (kPlanes == 2) st_shared_128(at + kBlockBytes, ql.x, ql.y, ql.z, ql.w);
         }
-    }
+    });
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
 
     const uint32_t tmem = sh.tmem_base, my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)col;
     uint32_t phase = 0;
+    const Descriptors desc;
     auto wait_done = [&] {
         if (!dead) {
             if (!mbar_wait(&sh.done, phase, &sh.abort, wait_limit)) {
@@ -323,59 +408,70 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         const NsSmallOp first = sh.ops[op0];
         if (first.kind == 1) {
             // ---- Gram: this CTA's columns, then the cluster's sum ----
-            float g[32];
+            float g[kCols];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) g[k] = 0.0f;
+            for (int k = 0; k < kCols; ++k) g[k] = 0.0f;
             // two planes: an accumulator takes 128 columns (its additions truncate, see ns_products.cu)
             const int chunk = kPlanes == 2 ? 2 : blocks;
             for (int b0 = 0; b0 < blocks; b0 += chunk) {
                 if (threadIdx.x == 0 && !dead && !withhold) {
                     for (int k = b0; k < min(b0 + chunk, blocks); ++k) {
-                        const uint32_t x = x_base + (uint32_t)(k * kPlanes * kBlockBytes);
+                        const uint64_t x = desc.rows(x_base + (uint32_t)(k * kPlanes * kBlockBytes));
                         issue_product<kPlanes, kPlanes>(tmem, x, x, false, k > b0);
                     }
                     tcgen05_commit<1>(&sh.done);
                 }
                 wait_done();
                 if (worker) {
-                    uint32_t v[32];
-                    tmem_ld_32x32_sync(my_tmem, v);
+                    float v[kCols];
+                    tmem_ld_16_sync(my_tmem, v);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) g[k] += __uint_as_float(v[k]);
+                    for (int k = 0; k < kCols; ++k) g[k] += v[k];
                 }
                 release();
             }
             if (clusters > 1) {
+                // f32 [64][64] as 1024 words of 16 bytes; every CTA sums its part of the words over the cluster, in
+                // rank order, and writes the sums to all (a word is read and rewritten by one thread only)
                 const uint32_t sums = square(kSumSquare);
-                const uint32_t mine = (uint32_t)(row * 64 + col) * 4;  // f32 [64][64]
+                const uint32_t mine = sums + (uint32_t)(row * 256);
                 if (worker) {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        st_shared_128(sums + mine + (uint32_t)((q ^ (lane & 7)) << 4), __float_as_uint(g[4 * q]), __float_as_uint(g[4 * q + 1]),
-                                      __float_as_uint(g[4 * q + 2]), __float_as_uint(g[4 * q + 3]));
+                    for (int q = 0; q < kCols / 4; ++q)
+                        st_shared_128(mine + (uint32_t)((((col >> 2) + q) ^ (row & 7)) << 4), __float_as_uint(g[4 * q]),
+                                      __float_as_uint(g[4 * q + 1]), __float_as_uint(g[4 * q + 2]), __float_as_uint(g[4 * q + 3]));
+                }
+                cluster_sync_all();
+                const int words = kSide * kSide / 4 / clusters;
+                for (int k = threadIdx.x; k < words; k += kThreads) {
+                    const uint32_t word = sums + (uint32_t)((rank * words + k) * 16);
+                    float4 part[kNsSmallCluster];
+#pragma unroll
+                    for (int r = 0; r < kNsSmallCluster; ++r)
+                        if (r < clusters) part[r] = ld_cluster_f32x4(map_to_cta(word, (uint32_t)r));
+                    float4 t = part[0];
+#pragma unroll
+                    for (int r = 1; r < kNsSmallCluster; ++r)
+                        if (r < clusters) t.x += part[r].x, t.y += part[r].y, t.z += part[r].z, t.w += part[r].w;
+#pragma unroll
+                    for (int r = 0; r < kNsSmallCluster; ++r)
+                        if (r < clusters) st_cluster_f32x4(map_to_cta(word, (uint32_t)r), t);
                 }
                 cluster_sync_all();
                 if (worker) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) g[k] = 0.0f;
-                    for (int r = 0; r < clusters; ++r) {
-                        const uint32_t from = map_to_cta(sums + mine, (uint32_t)r);
+                    for (int q = 0; q < kCols / 4; ++q) {
+                        uint32_t v[4];
+                        ld_shared_128(mine + (uint32_t)((((col >> 2) + q) ^ (row & 7)) << 4), v[0], v[1], v[2], v[3]);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            const float4 v = ld_cluster_f32x4(from + (uint32_t)((q ^ (lane & 7)) << 4));
-                            g[4 * q] += v.x;
-                            g[4 * q + 1] += v.y;
-                            g[4 * q + 2] += v.z;
-                            g[4 * q + 3] += v.w;
-                        }
+                        for (int e = 0; e < 4; ++e) g[4 * q + e] = __uint_as_float(v[e]);
                     }
                 }
-                cluster_sync_all();  // the sums' memory is a square again
             }
             if (worker) {
                 const float c = first.g * (first.scale_power == 2 ? scale * scale : 1.0f);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) g[k] *= c;
+                for (int k = 0; k < kCols; ++k) g[k] *= c;
                 put_row<2>(g, square(first.D), row, col);
             }
             release();
@@ -386,18 +482,17 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             while (!sh.ops[op1 - 1].stage_end) ++op1;
             if (threadIdx.x == 0 && !dead) {
                 for (int k = op0; k < op1; ++k)
-                    issue_product<2, 2>(tmem + (uint32_t)((k - op0) * 64), square(sh.ops[k].A), square(sh.ops[k].B), false, false);
+                    issue_product<2, 2>(tmem + (uint32_t)((k - op0) * 64), desc.rows(square(sh.ops[k].A)), desc.rows(square(sh.ops[k].B)), false, false);
                 tcgen05_commit<1>(&sh.done);
             }
             wait_done();
             if (worker) {
                 for (int k = op0; k < op1; ++k) {
                     const NsSmallOp op = sh.ops[k];
-                    uint32_t v[32];
-                    tmem_ld_32x32_sync(my_tmem + (uint32_t)((k - op0) * 64), v);
-                    float f[32];
+                    float f[kCols];
+                    tmem_ld_16_sync(my_tmem + (uint32_t)((k - op0) * 64), f);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) f[j] = op.g * __uint_as_float(v[j]);
+                    for (int j = 0; j < kCols; ++j) f[j] *= op.g;
                     if (op.E >= 0) add_row<2>(f, op.e, square(op.E), row, col);
                     if (op.F >= 0) add_row<2>(f, op.f, square(op.F), row, col);
                     put_row<2>(f, square(op.D), row, col);
@@ -406,57 +501,27 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             release();
             op0 = op1;
         } else {
-            // ---- update of X, four blocks of 64 columns at a time; the last one goes to the caller ----
-            const bool last = op0 + 1 == d.n_ops;
+            // ---- update of X, four blocks of 64 columns at a time, in place ----
             const float mult = first.scale_power == 1 ? scale : 1.0f;
-            const float out_scale = last ? d.final_scale : 1.0f;
-            const float ce = first.e * mult * out_scale, cg = first.g * mult * out_scale;
+            const float ce = first.e * mult, cg = first.g * mult;
             for (int b0 = 0; b0 < blocks; b0 += 4) {
                 const int b1 = min(b0 + 4, blocks);
                 if (threadIdx.x == 0 && !dead) {
                     for (int k = b0; k < b1; ++k)
-                        issue_product<2, kPlanes>(tmem + (uint32_t)((k - b0) * 64), square(first.A),
-                                                  x_base + (uint32_t)(k * kPlanes * kBlockBytes), true, false);
+                        issue_product<2, kPlanes>(tmem + (uint32_t)((k - b0) * 64), desc.rows(square(first.A)),
+                                                  desc.columns(x_base + (uint32_t)(k * kPlanes * kBlockBytes)), true, false);
                     tcgen05_commit<1>(&sh.done);
                 }
                 wait_done();
                 if (worker) {
                     for (int k = b0; k < b1; ++k) {
                         const uint32_t block = x_base + (uint32_t)(k * kPlanes * kBlockBytes);
-                        uint32_t v[32];
-                        tmem_ld_32x32_sync(my_tmem + (uint32_t)((k - b0) * 64), v);
-                        float f[32];
+                        float f[kCols];
+                        tmem_ld_16_sync(my_tmem + (uint32_t)((k - b0) * 64), f);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) f[j] = cg * __uint_as_float(v[j]);
+                        for (int j = 0; j < kCols; ++j) f[j] *= cg;
                         add_row<kPlanes>(f, ce, block, row, col);
-                        if (!last) {
-                            put_row<kPlanes>(f, block, row, col);
-                            continue;
-                        }
-                        if (dead || row >= d.n) continue;
-                        constexpr int kOut = kStep ? 2 : 1;
-                        const NsArray &dst = a.a[kOut];
-                        const int type = w.types[kOut];
-                        const bool vec = (a.direct >> kOut) & 1u, by_i = walks_i(dst);
-                        const float rate = w.rate * a.scale;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int j = s.j0 + k * 64 + col + q * 8;
-                            const int count = min(8, d.m - j);
-                            if (count <= 0) break;
-                            const int64_t at = (int64_t)row * dst.si + (int64_t)j * dst.sj;
-                            float o[8];
-                            if (kStep) {
-                                float p[8];
-                                load8(type, dst.ptr, at, dst.sj, count, vec && !by_i, p);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) o[e] = fmaf(-rate, f[q * 8 + e], p[e] * w.decay);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) o[e] = f[q * 8 + e];
-                            }
-                            store8(type, dst.ptr, at, dst.sj, count, vec && !by_i, o);
-                        }
+                        put_row<kPlanes>(f, block, row, col);
                     }
                 }
                 release();
@@ -465,6 +530,63 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         }
     }
 
+    // ---- from the last iterate to the caller ----
+    if (!dead) {
+        constexpr int kOut = kStep ? 2 : 1;
+        const NsArray &dst = a.a[kOut];
+        Share out = s;
+        out.along_i = walks_i(dst);
+        const float rate = w.rate * a.scale;
+        for (int o0 = threadIdx.x; o0 < out.octets(); o0 += kThreads * kInFlight) {
+            Raw p[kStep ? kInFlight : 1];
+#pragma unroll
+            for (int k = 0; k < (kStep ? kInFlight : 0); ++k) {
+                int i, j, count;
+                if (o0 + k * kThreads >= out.octets()) break;
+                out.locate(o0 + k * kThreads, i, j, count);
+                p[k].load(w.types[kOut], dst, out, (a.direct >> kOut) & 1u, i, j, count);
+            }
+#pragma unroll
+            for (int k = 0; k < kInFlight; ++k) {
+                int i, j, count;
+                if (o0 + k * kThreads >= out.octets()) break;
+                out.locate(o0 + k * kThreads, i, j, count);
+                if (count == 0) continue;
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+#pragma unroll
+                for (int pl = 0; pl < kPlanes; ++pl) {
+                    if (out.along_i) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            unsigned short h;
+                            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(x_address<kPlanes>(x_base, i + e, j) + pl * kBlockBytes) : "memory");
+                            f[e] += __half2float(__ushort_as_half(h));
+                        }
+                    } else {
+                        uint32_t v[4];
+                        ld_shared_128(x_address<kPlanes>(x_base, i, j) + pl * kBlockBytes, v[0], v[1], v[2], v[3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 x = unpack_half(v[e]);
+                            f[2 * e] += x.x, f[2 * e + 1] += x.y;
+                        }
+                    }
+                }
+                if (kStep) {
+                    float pp[8];
+                    p[kStep ? k : 0].get(w.types[kOut], dst, out, i, j, count, pp);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = fmaf(-rate, f[e] * d.final_scale, pp[e] * w.decay);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= d.final_scale;
+                }
+                out.write(w.types[kOut], dst, (a.direct >> kOut) & 1u, i, j, count, f);
+            }
+        }
+    }
     tcgen05_fence_before();
     __syncthreads();
     cluster_sync_all();  // nobody leaves while its shared memory may be read
