@@ -217,7 +217,7 @@ std::vector<NsSmallOp> small_program(const Schedule &s)
         for (size_t k = 0; k < stage.size(); ++k) {
             const Product &p = stage[k];
             ops.push_back({square(p.A), square(p.B), square(p.E), square(p.F), square(p.D), (int8_t)(p.update ? 2 : p.gram ? 1 : 0),
-                           (int8_t)(k + 1 == stage.size()), (int8_t)p.scale_power, (float)p.e, (float)p.f, (float)p.g});
+                           (int8_t)(stage.size() - k), (int8_t)p.scale_power, (float)p.e, (float)p.f, (float)p.g, {}});
         }
     return ops;
 }
@@ -289,6 +289,9 @@ struct vb_ns_plan {
     std::vector<Batch> batches;
     std::vector<int32_t> small_matrices;  // those that ns_small.cu runs, in its order
     vb::NsSmall small{};
+    // where a plan has matrices of both kinds, the small ones run beside the others
+    cudaStream_t side = nullptr;
+    cudaEvent_t forked = nullptr, joined = nullptr;
     vb::NsError error{};
     uint32_t *h_error = nullptr;
     bool withhold = false;
@@ -312,6 +315,9 @@ namespace {
 void free_plan(vb_ns_plan *p)
 {
     if (p->d_base) cudaFree(p->d_base);
+    if (p->forked) cudaEventDestroy(p->forked);
+    if (p->joined) cudaEventDestroy(p->joined);
+    if (p->side) cudaStreamDestroy(p->side);
     if (p->h_error) cudaFreeHost(p->h_error);
     delete p;
 }
@@ -529,19 +535,23 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         p->shape = pick_shape(problems, stage_begin, p->eng->sm_count);
         tile_list.clear();
         std::vector<uint32_t> done((size_t)n, 0), stage_done((size_t)n, 0);
+        size_t widest = 0;
         for (size_t k = 0; k < n_stages; ++k) {
+            const size_t stage_at = tile_list.size();
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
                 const size_t i = (size_t)problems[q].matrix;
                 stage_done[i] += for_tiles(problems[q], p->shape, [&](int m0, int n0, bool mirror) {
                     tile_list.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, done[i], 0});
                 });
             }
+            widest = std::max(widest, tile_list.size() - stage_at);
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) done[(size_t)problems[q].matrix] = stage_done[(size_t)problems[q].matrix];
         }
         NsProduct *d_problems = c.take<NsProduct>(problems.size());
         NsTile *d_tiles = c.take<NsTile>(tile_list.size());
         if (tile_list.size() > (size_t)INT32_MAX) return fail(VB_ERR_UNSUPPORTED, "the plan's products have too many tiles");
-        p->products = {d_problems, d_tiles, p->ew.stored, (int)tile_list.size()};
+        // more CTAs (pairs) than the largest stage has tiles would mostly wait, on SMs that others could use
+        p->products = {d_problems, d_tiles, p->ew.stored, (int)tile_list.size(), (int)widest};
         if (round == 1) {
             VB_CUDA(cudaMemcpyAsync(d_problems, problems.data(), problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
@@ -569,6 +579,11 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             VB_CUDA(cudaMemcpyAsync(d_tile_matrix, tile_matrix.data(), tile_matrix.size() * sizeof(int32_t), cudaMemcpyHostToDevice, p->eng->stream));
         }
     }
+    if (!small.empty() && p->products.n_tiles > 0) {
+        VB_CUDA(cudaStreamCreateWithFlags(&p->side, cudaStreamNonBlocking));
+        VB_CUDA(cudaEventCreateWithFlags(&p->forked, cudaEventDisableTiming));
+        VB_CUDA(cudaEventCreateWithFlags(&p->joined, cudaEventDisableTiming));
+    }
     VB_CUDA(cudaHostAlloc((void **)&p->h_error, sizeof(uint32_t), cudaHostAllocMapped));
     *p->h_error = 0;
     VB_CUDA(cudaHostGetDevicePointer((void **)&p->error.host, p->h_error, 0));
@@ -590,6 +605,23 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
         for (int32_t k = 0; k < b.count; ++k) fill(b.first + k, args.m[k]);
     };
     const uint32_t wait_limit = p->wait_limit ? p->wait_limit : p->default_wait_limit;
+    cudaStream_t side = e->stream;
+    if (p->side) {
+        side = p->side;
+        VB_CUDA(cudaEventRecord(p->forked, e->stream));
+        VB_CUDA(cudaStreamWaitEvent(side, p->forked, 0));
+    }
+    if (!p->side && !p->small_matrices.empty()) prof_begin(e, VB_PHASE_MUON_NS);
+    for (size_t k0 = 0; k0 < p->small_matrices.size(); k0 += kNsBatch) {
+        args.first = (int32_t)k0;
+        args.count = (int32_t)std::min<size_t>(kNsBatch, p->small_matrices.size() - k0);
+        for (int32_t k = 0; k < args.count; ++k) fill(p->small_matrices[k0 + (size_t)k], args.m[k]);
+        VB_TRY(launch_ns_small(w, p->small, args, p->error, step, side, wait_limit, p->withhold));
+        e->launches += 1;
+        p->withhold = false;
+    }
+    if (!p->side && !p->small_matrices.empty()) prof_end(e, VB_PHASE_MUON_NS);
+    if (p->side) VB_CUDA(cudaEventRecord(p->joined, side));
     prof_begin(e, VB_PHASE_MUON_PRE);
     for (const auto &b : p->batches) {
         if (b.n_tiles == 0) continue;
@@ -599,22 +631,14 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
         e->launches += 2;
     }
     prof_end(e, VB_PHASE_MUON_PRE);
-    prof_begin(e, VB_PHASE_MUON_NS);
     if (p->products.n_tiles > 0) {
+        prof_begin(e, VB_PHASE_MUON_NS);
         VB_TRY(launch_ns_products(p->products, p->shape, p->planes, w.active, p->error, e->sm_count, e->stream, wait_limit, p->withhold));
         e->launches += 1;
         p->withhold = false;
-    }
-    for (size_t k0 = 0; k0 < p->small_matrices.size(); k0 += kNsBatch) {
-        args.first = (int32_t)k0;
-        args.count = (int32_t)std::min<size_t>(kNsBatch, p->small_matrices.size() - k0);
-        for (int32_t k = 0; k < args.count; ++k) fill(p->small_matrices[k0 + (size_t)k], args.m[k]);
-        VB_TRY(launch_ns_small(w, p->small, args, p->error, step, e->stream, wait_limit, p->withhold));
-        e->launches += 1;
-        p->withhold = false;
+        prof_end(e, VB_PHASE_MUON_NS);
     }
     p->wait_limit = 0;
-    prof_end(e, VB_PHASE_MUON_NS);
     prof_begin(e, VB_PHASE_MUON_APPLY);
     for (const auto &b : p->batches) {
         if (b.n_tiles == 0) continue;
@@ -623,6 +647,7 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
         e->launches += 1;
     }
     prof_end(e, VB_PHASE_MUON_APPLY);
+    if (p->side) VB_CUDA(cudaStreamWaitEvent(e->stream, p->joined, 0));
     return VB_OK;
 }
 
@@ -749,6 +774,7 @@ int vb_ns_plan_destroy(vb_ns_plan *p)
     cudaSetDevice(p->device);
     if (p->eng) {
         cudaStreamSynchronize(p->eng->stream);
+        if (p->side) cudaStreamSynchronize(p->side);  // a call that failed half-way may not have joined it
         auto &all = p->eng->ns_plans;
         all.erase(std::remove(all.begin(), all.end(), p), all.end());
     }

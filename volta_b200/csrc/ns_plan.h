@@ -51,6 +51,7 @@ struct NsLaunch {
     const NsTile *tiles;
     uint32_t *stored;  // per matrix: epilogue warps' arrivals, zeroed by the gather pass
     int n_tiles;
+    int widest;        // tiles of the largest stage
 };
 
 // Tile shapes of the product kernel.
@@ -127,12 +128,13 @@ constexpr int kNsSmallSide = 64;
 constexpr int kNsSmallOps = 128;     // longest program
 constexpr int kNsSmallSquares = 5;
 constexpr int kNsSmallCluster = 8;   // most CTAs of one matrix
-struct NsSmallOp {
+struct alignas(16) NsSmallOp {
     int8_t A, B, E, F, D;   // short-side matrices (0 ..), -1: none; of a Gram D, of an update A only
     int8_t kind;            // 0 product of two short-side matrices, 1 Gram, 2 update of X
-    int8_t stage_end;       // the next op depends on this one
+    int8_t stage_ops;       // products of this op's stage from this one on
     int8_t scale_power;
     float e, f, g;          // as in NsProduct
+    int32_t pad[3];
 };
 struct NsSmallMatrix {
     int32_t n, m;

@@ -644,7 +644,7 @@ int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, i
         }
         resident = std::min(sm_count, 2 * max_clusters);
     }
-    const int groups = std::min(resident / kCtas, l.n_tiles);
+    const int groups = std::min(resident / kCtas, l.widest);
     cfg.gridDim = dim3((unsigned)(groups * kCtas));
     VB_CUDA(cudaLaunchKernelEx(&cfg, ns_product_kernel<kCtas, kPlanes>, l, d_active, error, wait_limit, withhold ? 1 : 0));
     return VB_OK;

@@ -102,9 +102,9 @@ __device__ __forceinline__ void put_row(float (&f)[kCols], uint32_t block, int r
 
 // A (128 x 64, rows from 64 on unused) times B (64 x 64) into 64 accumulator columns; operands are blocks of
 // kA and kB planes, the products of their planes smallest first.  `a` and `b` are descriptors of plane 0 (see
-// Descriptors): other planes and k slices are reached by adding to the address field.
+// Descriptors): other planes and k slices are reached by adding to the address field.  k_slices: 16 each.
 template <int kA, int kB>
-__device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_t b, bool b_mn, bool accumulate)
+__device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_t b, bool b_mn, bool accumulate, int k_slices)
 {
     // f32 accumulator, f16 operands, A K-major, M = 128, N = 64
     const uint32_t idesc = (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(kSide >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -117,8 +117,8 @@ __device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_
         for (int pa = 0; pa < kA; ++pa) {
             const int pb = t - pa;
             if (pb < 0 || pb >= kB) continue;
-#pragma unroll
-            for (int kk = 0; kk < kSide / 16; ++kk) {
+#pragma unroll 1
+            for (int kk = 0; kk < k_slices; ++kk) {
                 tcgen05_mma_bf16<1>(tmem, a + (uint32_t)(pa * (kBlockBytes >> 4) + kk * (32 >> 4)),
                                     b + (uint32_t)(pb * (kBlockBytes >> 4)) + kk * step_b, idesc, keep);
                 keep = 1u;
@@ -277,7 +277,21 @@ __device__ __forceinline__ void for_u(const NsElementwise &w, const NsMatrixArg 
     }
 }
 
-// 8 values of the planes of X in shared memory, along i (i a multiple of 8) or along j
+// h[e] <- h[(e + turn) mod 8], turn in 0 .. 8
+__device__ __forceinline__ void rotate8(__half (&h)[8], int turn)
+{
+#pragma unroll
+    for (int bit = 1; bit < 8; bit *= 2) {
+        const bool move = (turn & bit) != 0;
+        __half r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = move ? h[(e + bit) & 7] : h[e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = r[e];
+    }
+}
+
+// Where element (i, j) of X lies in shared memory (plane 0)
 template <int kPlanes>
 __device__ __forceinline__ uint32_t x_address(uint32_t x_base, int i, int j)
 {
@@ -365,9 +379,14 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             l[e] = __float2half_rn(x - __half2float(h[e]));
         }
         if (s.along_i) {
+            // lanes of a warp hold different groups of 8 rows and the same few columns: in step e a lane stores its
+            // row (e + group) mod 8, so that their 16-byte parts, which the swizzle places by row mod 8, differ
+            const int turn = (i >> 3) & 7;
+            rotate8(h, turn);
+            if (kPlanes == 2) rotate8(l, turn);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t at = x_address<kPlanes>(x_base, i + e, j);
+                const uint32_t at = x_address<kPlanes>(x_base, i + ((e + turn) & 7), j);
                 asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(h[e])) : "memory");
                 if (kPlanes == 2) asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + kBlockBytes), "h"(__half_as_ushort(l[e])) : "memory");
             }
@@ -384,6 +403,8 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     const uint32_t tmem = sh.tmem_base, my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)col;
     uint32_t phase = 0;
     const Descriptors desc;
+    const bool issuer = threadIdx.x == 96;    // of a warp that does not drain
+    const int k_slices = (d.n + 15) / 16;     // of products over the short side
     auto wait_done = [&] {
         if (!dead) {
             if (!mbar_wait(&sh.done, phase, &sh.abort, wait_limit)) {
@@ -414,10 +435,10 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             // two planes: an accumulator takes 128 columns (its additions truncate, see ns_products.cu)
             const int chunk = kPlanes == 2 ? 2 : blocks;
             for (int b0 = 0; b0 < blocks; b0 += chunk) {
-                if (threadIdx.x == 0 && !dead && !withhold) {
+                if (issuer && !dead && !withhold) {
                     for (int k = b0; k < min(b0 + chunk, blocks); ++k) {
                         const uint64_t x = desc.rows(x_base + (uint32_t)(k * kPlanes * kBlockBytes));
-                        issue_product<kPlanes, kPlanes>(tmem, x, x, false, k > b0);
+                        issue_product<kPlanes, kPlanes>(tmem, x, x, false, k > b0, kSide / 16);
                     }
                     tcgen05_commit<1>(&sh.done);
                 }
@@ -478,38 +499,51 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             op0 += 1;
         } else if (first.kind == 0) {
             // ---- one stage: one or two independent products ----
-            int op1 = op0 + 1;
-            while (!sh.ops[op1 - 1].stage_end) ++op1;
-            if (threadIdx.x == 0 && !dead) {
-                for (int k = op0; k < op1; ++k)
-                    issue_product<2, 2>(tmem + (uint32_t)((k - op0) * 64), desc.rows(square(sh.ops[k].A)), desc.rows(square(sh.ops[k].B)), false, false);
+            const int count = first.stage_ops;
+            if (issuer && !dead) {
+                for (int k = 0; k < count; ++k)
+                    issue_product<2, 2>(tmem + (uint32_t)(k * 64), desc.rows(square(sh.ops[op0 + k].A)),
+                                        desc.rows(square(sh.ops[op0 + k].B)), false, false, k_slices);
                 tcgen05_commit<1>(&sh.done);
+            }
+            // the terms that are there already, while the products run
+            float f[2][kCols];
+            if (worker) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) f[k][j] = 0.0f;
+                    if (k >= count) continue;
+                    const NsSmallOp op = sh.ops[op0 + k];
+                    if (op.E >= 0) add_row<2>(f[k], op.e, square(op.E), row, col);
+                    if (op.F >= 0) add_row<2>(f[k], op.f, square(op.F), row, col);
+                }
             }
             wait_done();
             if (worker) {
-                for (int k = op0; k < op1; ++k) {
-                    const NsSmallOp op = sh.ops[k];
-                    float f[kCols];
-                    tmem_ld_16_sync(my_tmem + (uint32_t)((k - op0) * 64), f);
 #pragma unroll
-                    for (int j = 0; j < kCols; ++j) f[j] *= op.g;
-                    if (op.E >= 0) add_row<2>(f, op.e, square(op.E), row, col);
-                    if (op.F >= 0) add_row<2>(f, op.f, square(op.F), row, col);
-                    put_row<2>(f, square(op.D), row, col);
+                for (int k = 0; k < 2; ++k) {
+                    if (k >= count) continue;
+                    float v[kCols];
+                    tmem_ld_16_sync(my_tmem + (uint32_t)(k * 64), v);
+                    const float c = sh.ops[op0 + k].g;
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) f[k][j] = fmaf(c, v[j], f[k][j]);
+                    put_row<2>(f[k], square(sh.ops[op0 + k].D), row, col);
                 }
             }
             release();
-            op0 = op1;
+            op0 += count;
         } else {
             // ---- update of X, four blocks of 64 columns at a time, in place ----
             const float mult = first.scale_power == 1 ? scale : 1.0f;
             const float ce = first.e * mult, cg = first.g * mult;
             for (int b0 = 0; b0 < blocks; b0 += 4) {
                 const int b1 = min(b0 + 4, blocks);
-                if (threadIdx.x == 0 && !dead) {
+                if (issuer && !dead) {
                     for (int k = b0; k < b1; ++k)
                         issue_product<2, kPlanes>(tmem + (uint32_t)((k - b0) * 64), desc.rows(square(first.A)),
-                                                  desc.columns(x_base + (uint32_t)(k * kPlanes * kBlockBytes)), true, false);
+                                                  desc.columns(x_base + (uint32_t)(k * kPlanes * kBlockBytes)), true, false, k_slices);
                     tcgen05_commit<1>(&sh.done);
                 }
                 wait_done();
@@ -557,13 +591,21 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 for (int e = 0; e < 8; ++e) f[e] = 0.0f;
 #pragma unroll
                 for (int pl = 0; pl < kPlanes; ++pl) {
-                    if (out.along_i) {
+                    if (out.along_i) {  // as the stores above, the other way round
+                        const int turn = (i >> 3) & 7;
+                        __half h[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            unsigned short h;
-                            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(x_address<kPlanes>(x_base, i + e, j) + pl * kBlockBytes) : "memory");
-                            f[e] += __half2float(__ushort_as_half(h));
+                            unsigned short x;
+                            asm volatile("ld.shared.b16 %0, [%1];"
+                                         : "=h"(x)
+                                         : "r"(x_address<kPlanes>(x_base, i + ((e + turn) & 7), j) + pl * kBlockBytes)
+                                         : "memory");
+                            h[e] = __ushort_as_half(x);
                         }
+                        rotate8(h, 8 - turn);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] += __half2float(h[e]);
                     } else {
                         uint32_t v[4];
                         ld_shared_128(x_address<kPlanes>(x_base, i, j) + pl * kBlockBytes, v[0], v[1], v[2], v[3]);
