@@ -141,6 +141,20 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
     return ti;
 }
 
+__device__ __forceinline__ Tile uniform_tile(const Tile &t)
+{
+    Tile u;
+    u.p = uniform(const_cast<NsProduct *>(t.p));
+    u.m0 = uniform(t.m0);
+    u.n0 = uniform(t.n0);
+    u.k_blocks = uniform(t.k_blocks);
+    u.matrix = uniform(t.matrix);
+    u.after = uniform(t.after);
+    const int flags = uniform((t.mirror ? 1 : 0) | (t.b_mn ? 2 : 0) | (t.skipped ? 4 : 0));
+    u.mirror = flags & 1, u.b_mn = flags & 2, u.skipped = flags & 4;
+    return u;
+}
+
 __device__ __forceinline__ uint32_t load_acquire(const uint32_t *p)
 {
     uint32_t v;
@@ -312,7 +326,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     Barriers *bars = reinterpret_cast<Barriers *>(epi_stage + kEpiWarps * kEpiWarpBytes);
     volatile uint32_t *abort_flag = &bars->abort;
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = uniform((int)(threadIdx.x >> 5));
     const int lane = threadIdx.x & 31;
     const uint32_t cta_rank = kCtas == 2 ? cluster_ctarank() : 0u;
     const int group_id = blockIdx.x / kCtas;
@@ -358,67 +372,70 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
 
     if (warp == 0) {
         // ---- TMA producer ----
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            const uint32_t slots = smem_u32(smem), empty0 = smem_u32(&bars->empty[0]);
-            // the leader announces the bytes of both CTAs; the peer's may land before that, the phase cannot end before it
-            const uint32_t full0 = kCtas == 2 ? map_to_cta(smem_u32(&bars->full[0]), 0) : smem_u32(&bars->full[0]);
-            Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
-            for (int t = group_id; t < n_tiles && ok; t += n_groups) {
-                const Tile ti = next;
-                next = fetch_tile(launch, active, t + n_groups);
-                if (ti.skipped) continue;
-                const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * 128;
-                const int plane_rows = ti.p->plane_rows;
-                const CUtensorMap *map_a = &ti.p->map_a, *map_b = &ti.p->map_b;
-                if (!wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device, abort_flag, wait_limit)) {
+        const bool elected = elect_one();
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const uint32_t slots = uniform(smem_u32(smem)), empty0 = uniform(smem_u32(&bars->empty[0]));
+        // the leader announces the bytes of both CTAs; the peer's may land before that, the phase cannot end before it
+        const uint32_t my_full0 = uniform(smem_u32(&bars->full[0]));
+        const uint32_t full0 = uniform(kCtas == 2 ? map_to_cta(my_full0, 0) : my_full0);
+        Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
+        for (int t = group_id; t < n_tiles && ok; t += n_groups) {
+            const Tile ti = uniform_tile(next);
+            next = fetch_tile(launch, active, t + n_groups);
+            if (ti.skipped) continue;
+            const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * 128;
+            const int plane_rows = uniform(ti.p->plane_rows);
+            const CUtensorMap *map_a = &ti.p->map_a, *map_b = &ti.p->map_b;
+            if (!__all_sync(0xffffffffu, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device, abort_flag,
+                                                     wait_limit))) {
+                ok = false;
+                break;
+            }
+            asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what other SMs stored
+#pragma unroll 1
+            for (int kb = 0; kb < ti.k_blocks; ++kb) {
+                if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, wait_limit))) {
                     ok = false;
                     break;
                 }
-                asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what other SMs stored
-#pragma unroll 1
-                for (int kb = 0; kb < ti.k_blocks; ++kb) {
-                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, wait_limit)) {
-                        ok = false;
-                        break;
-                    }
-                    if (!withhold) {  // withheld: nothing is announced or staged, the bounded waits run out
-                        const uint32_t slot = slots + (uint32_t)stage * C::kStageBytes, full = full0 + 8 * stage;
-                        if (cta_rank == 0) mbar_expect_tx(&bars->full[stage], kCtas * C::kStageBytes);
+                if (elected && !withhold) {  // withheld: nothing is announced or staged, the bounded waits run out
+                    const uint32_t slot = slots + (uint32_t)stage * C::kStageBytes, full = full0 + 8 * stage;
+                    if (cta_rank == 0) mbar_expect_tx(my_full0 + 8 * stage, kCtas * C::kStageBytes);
 #pragma unroll
-                        for (int pl = 0; pl < kPlanes; ++pl) {
-                            load_rows<kCtas>(slot + pl * C::kPlaneBytes, map_a, false, a_row0, kb * BK, pl * plane_rows, full);
-                            load_rows<kCtas>(slot + pl * C::kPlaneBytes + kRows128Bytes, map_b, ti.b_mn, b_row0, kb * BK,
-                                             pl * plane_rows, full);
-                        }
-                    }
-                    if (++stage == C::kStages) {
-                        stage = 0;
-                        phase ^= 1u;
+                    for (int pl = 0; pl < kPlanes; ++pl) {
+                        load_rows<kCtas>(slot + pl * C::kPlaneBytes, map_a, false, a_row0, kb * BK, pl * plane_rows, full);
+                        load_rows<kCtas>(slot + pl * C::kPlaneBytes + kRows128Bytes, map_b, ti.b_mn, b_row0, kb * BK,
+                                         pl * plane_rows, full);
                     }
                 }
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
-            if (!ok) {
-                bars->abort = 1;
-                report(error, 1u);
-            }
+        }
+        if (!ok && lane == 0) {
+            bars->abort = 1;
+            report(error, 1u);
         }
         __syncwarp();
     } else if (warp == 1) {
         // ---- MMA issuer (leader CTA) ----
-        if (lane == 0 && cta_rank == 0) {
+        if (cta_rank == 0) {
+            const bool elected = elect_one();
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
-            // One thread feeds the tensor core: what it computes per MMA must stay small, so descriptors are made
-            // once (for slot 0) and moved by adding 16-byte units to their address field.
-            const uint64_t desc_k = operand_desc(smem_u32(smem), false, 0), desc_mn = operand_desc(smem_u32(smem), true, 0);
-            const uint32_t full0 = smem_u32(&bars->full[0]);
+            // descriptors are made once (for slot 0) and moved by adding 16-byte units to their address field
+            const uint32_t base = uniform(smem_u32(smem));
+            const uint64_t desc_k = operand_desc(base, false, 0), desc_mn = operand_desc(base, true, 0);
+            const uint32_t full0 = uniform(smem_u32(&bars->full[0])), empty0 = uniform(smem_u32(&bars->empty[0]));
+            const uint32_t tmem = uniform(tmem_base);
             Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
             for (int t = group_id; t < n_tiles && ok; t += n_groups) {
-                const Tile ti = next;
+                const Tile ti = uniform_tile(next);
                 next = fetch_tile(launch, active, t + n_groups);
                 if (ti.skipped) continue;
                 const uint32_t idesc = make_idesc(ti.b_mn, BM * kCtas, C::BN);
@@ -427,46 +444,47 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 const uint32_t step_b = ti.b_mn ? 2048 >> 4 : 32 >> 4;
                 for (int k0 = 0; k0 < ti.k_blocks && ok; k0 += C::kChunkBlocks) {
                     const int k1 = min(k0 + C::kChunkBlocks, ti.k_blocks);
-                    if (!mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, wait_limit)) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, wait_limit))) {
                         ok = false;
                         break;
                     }
                     tcgen05_fence_after();
-                    const uint32_t tmem_d = tmem_base + (uint32_t)(acc * C::BN);
+                    const uint32_t tmem_d = tmem + (uint32_t)(acc * C::BN);
 #pragma unroll 1
                     for (int kb = k0; kb < k1; ++kb) {
-                        if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, wait_limit)) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * stage, phase, abort_flag, wait_limit))) {
                             ok = false;
                             break;
                         }
                         tcgen05_fence_after();
                         const uint32_t slot = (uint32_t)stage * (C::kStageBytes >> 4);
-                        // two planes: three products, smallest first; the dropped low x low is below 2^-22
+                        if (elected) {
+                            // two planes: three products, smallest first; the dropped low x low is below 2^-22
 #pragma unroll
-                        for (int term = 0; term < (kPlanes == 2 ? 3 : 1); ++term) {
-                            const uint64_t da = desc_k + slot + (kPlanes == 2 && term == 1 ? C::kPlaneBytes >> 4 : 0);
-                            const uint64_t db = desc_b0 + slot + (kRows128Bytes >> 4) +
-                                                (kPlanes == 2 && term == 0 ? C::kPlaneBytes >> 4 : 0);
+                            for (int term = 0; term < (kPlanes == 2 ? 3 : 1); ++term) {
+                                const uint64_t da = desc_k + slot + (kPlanes == 2 && term == 1 ? C::kPlaneBytes >> 4 : 0);
+                                const uint64_t db = desc_b0 + slot + (kRows128Bytes >> 4) +
+                                                    (kPlanes == 2 && term == 0 ? C::kPlaneBytes >> 4 : 0);
 #pragma unroll
-                            for (int kk = 0; kk < BK / UMMA_K; ++kk)
-                                tcgen05_mma_bf16<kCtas>(tmem_d, da + kk * (32 >> 4), db + kk * step_b, idesc,
-                                                        (kb > k0 || term > 0 || kk > 0) ? 1u : 0u);
+                                for (int kk = 0; kk < BK / UMMA_K; ++kk)
+                                    tcgen05_mma_bf16<kCtas>(tmem_d, da + kk * (32 >> 4), db + kk * step_b, idesc,
+                                                            (kb > k0 || term > 0 || kk > 0) ? 1u : 0u);
+                            }
+                            tcgen05_commit<kCtas>(empty0 + 8 * stage);
+                            if (kb + 1 == k1) tcgen05_commit<kCtas>(&bars->tmem_full[acc]);
                         }
-                        tcgen05_commit<kCtas>(&bars->empty[stage]);
+                        __syncwarp();
                         if (++stage == C::kStages) {
                             stage = 0;
                             phase ^= 1u;
                         }
                     }
                     if (!ok) break;
-                    tcgen05_commit<kCtas>(&bars->tmem_full[acc]);
-                    if (++acc == 2) {
-                        acc = 0;
-                        acc_phase ^= 1u;
-                    }
+                    acc ^= 1;
+                    acc_phase ^= acc == 0 ? 1u : 0u;
                 }
             }
-            if (!ok) {
+            if (!ok && lane == 0) {
                 bars->abort = 1;
                 report(error, 2u);
             }
@@ -564,7 +582,6 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             if (ok) {  // this warp's part of D is in memory, for TMA loads of other SMs
                 if (lane == 0) {
                     bulk_wait_all();
-                    asm volatile("fence.proxy.async;" ::: "memory");
                     asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(launch.stored + ti.matrix) : "memory");
                 }
                 __syncwarp();

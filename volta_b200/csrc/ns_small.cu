@@ -102,9 +102,11 @@ __device__ __forceinline__ void put_row(float (&f)[kCols], uint32_t block, int r
 
 // A (128 x 64, rows from 64 on unused) times B (64 x 64) into 64 accumulator columns; operands are blocks of
 // kA and kB planes, the products of their planes smallest first.  `a` and `b` are descriptors of plane 0 (see
-// Descriptors): other planes and k slices are reached by adding to the address field.  k_slices: 16 each.
+// Descriptors): other planes and k slices are reached by adding to the address field.  k_slices: 16 each.  The whole
+// warp runs this, its elected lane issues.
 template <int kA, int kB>
-__device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_t b, bool b_mn, bool accumulate, int k_slices)
+__device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_t b, bool b_mn, bool accumulate, int k_slices,
+                                              bool elected)
 {
     // f32 accumulator, f16 operands, A K-major, M = 128, N = 64
     const uint32_t idesc = (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(kSide >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -119,8 +121,9 @@ __device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_
             if (pb < 0 || pb >= kB) continue;
 #pragma unroll 1
             for (int kk = 0; kk < k_slices; ++kk) {
-                tcgen05_mma_bf16<1>(tmem, a + (uint32_t)(pa * (kBlockBytes >> 4) + kk * (32 >> 4)),
-                                    b + (uint32_t)(pb * (kBlockBytes >> 4)) + kk * step_b, idesc, keep);
+                if (elected)
+                    tcgen05_mma_bf16<1>(tmem, a + (uint32_t)(pa * (kBlockBytes >> 4) + kk * (32 >> 4)),
+                                        b + (uint32_t)(pb * (kBlockBytes >> 4)) + kk * step_b, idesc, keep);
                 keep = 1u;
             }
         }
@@ -322,7 +325,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     const NsMatrixArg &a = b.m[index];
     const NsSmallMatrix d = small.matrices[b.first + index];
     if (a.live == 0u) return;  // the whole cluster
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const bool worker = (warp & 3) < 2;  // TMEM lanes 0 .. 63
     const int row = (warp & 3) * 32 + lane, col = (warp >> 2) * kCols;
 
@@ -400,11 +403,12 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
 
-    const uint32_t tmem = sh.tmem_base, my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)col;
+    const uint32_t tmem = uniform(sh.tmem_base), my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)col;
     uint32_t phase = 0;
     const Descriptors desc;
-    const bool issuer = threadIdx.x == 96;    // of a warp that does not drain
-    const int k_slices = (d.n + 15) / 16;     // of products over the short side
+    const bool issuer = warp == 3;            // a warp that does not drain; one lane of it issues
+    const bool elected = issuer && elect_one();
+    const int k_slices = uniform((d.n + 15) / 16);     // of products over the short side
     auto wait_done = [&] {
         if (!dead) {
             if (!mbar_wait(&sh.done, phase, &sh.abort, wait_limit)) {
@@ -438,9 +442,9 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 if (issuer && !dead && !withhold) {
                     for (int k = b0; k < min(b0 + chunk, blocks); ++k) {
                         const uint64_t x = desc.rows(x_base + (uint32_t)(k * kPlanes * kBlockBytes));
-                        issue_product<kPlanes, kPlanes>(tmem, x, x, false, k > b0, kSide / 16);
+                        issue_product<kPlanes, kPlanes>(tmem, x, x, false, k > b0, kSide / 16, elected);
                     }
-                    tcgen05_commit<1>(&sh.done);
+                    if (elected) tcgen05_commit<1>(&sh.done);
                 }
                 wait_done();
                 if (worker) {
@@ -502,9 +506,9 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             const int count = first.stage_ops;
             if (issuer && !dead) {
                 for (int k = 0; k < count; ++k)
-                    issue_product<2, 2>(tmem + (uint32_t)(k * 64), desc.rows(square(sh.ops[op0 + k].A)),
-                                        desc.rows(square(sh.ops[op0 + k].B)), false, false, k_slices);
-                tcgen05_commit<1>(&sh.done);
+                    issue_product<2, 2>(tmem + (uint32_t)(k * 64), desc.rows(square(uniform((int)sh.ops[op0 + k].A))),
+                                        desc.rows(square(uniform((int)sh.ops[op0 + k].B))), false, false, k_slices, elected);
+                if (elected) tcgen05_commit<1>(&sh.done);
             }
             // the terms that are there already, while the products run
             float f[2][kCols];
@@ -542,9 +546,9 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 const int b1 = min(b0 + 4, blocks);
                 if (issuer && !dead) {
                     for (int k = b0; k < b1; ++k)
-                        issue_product<2, kPlanes>(tmem + (uint32_t)((k - b0) * 64), desc.rows(square(first.A)),
-                                                  desc.columns(x_base + (uint32_t)(k * kPlanes * kBlockBytes)), true, false, k_slices);
-                    tcgen05_commit<1>(&sh.done);
+                        issue_product<2, kPlanes>(tmem + (uint32_t)((k - b0) * 64), desc.rows(square(uniform((int)first.A))),
+                                                  desc.columns(x_base + (uint32_t)(k * kPlanes * kBlockBytes)), true, false, k_slices, elected);
+                    if (elected) tcgen05_commit<1>(&sh.done);
                 }
                 wait_done();
                 if (worker) {

@@ -14,11 +14,11 @@ __device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
 }
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes)
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes)  // shared-memory address
 {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) { mbar_expect_tx(smem_u32(bar), bytes); }
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -49,6 +49,31 @@ __device__ __forceinline__ bool mbar_wait(Bar bar, uint32_t parity, volatile uin
         if ((i & 63u) == 63u && *abort_flag != 0u) return false;
     }
     return false;
+}
+
+// True in one lane of a converged warp.  tcgen05 and TMA instructions take their descriptors and addresses from
+// uniform registers: a role whose whole warp runs the loop and only predicates these instructions keeps
+// everything there, one that branches to a single lane moves every operand over for every instruction (80 to
+// 120 cycles per tcgen05.mma).
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0u;
+}
+// A value that is the same in all lanes, in a form the compiler knows to be so.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+template <typename T>
+__device__ __forceinline__ T *uniform(T *p)
+{
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = uniform((uint32_t)v), hi = uniform((uint32_t)(v >> 32));
+    return reinterpret_cast<T *>(((uint64_t)hi << 32) | lo);
 }
 
 __device__ __forceinline__ uint32_t cluster_ctarank()
@@ -137,16 +162,21 @@ __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fe
 
 // Arrive on `bar` (same offset in every CTA of the group) once all MMAs issued so far are done.
 template <int kCtas>
-__device__ __forceinline__ void tcgen05_commit(uint64_t *bar)
+__device__ __forceinline__ void tcgen05_commit(uint32_t bar)
 {
     if (kCtas == 2)
         asm volatile(
             "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-            ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+            ::"r"(bar), "h"((uint16_t)3)
             : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                      : "memory");
+}
+template <int kCtas>
+__device__ __forceinline__ void tcgen05_commit(uint64_t *bar)
+{
+    tcgen05_commit<kCtas>(smem_u32(bar));
 }
 template <int kCtas>
 __device__ __forceinline__ void tcgen05_mma_bf16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
