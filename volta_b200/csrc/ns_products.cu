@@ -62,7 +62,7 @@ constexpr int kFirstEpiWarp = 2;  // warp 0 produces, warp 1 issues
 constexpr int kThreads = (kFirstEpiWarp + kEpiWarps) * 32;
 constexpr int kPieceCols = 64;
 constexpr int kPieceBytes = 32 * kPieceCols * 2;  // 32 rows of 128 bytes, 16-byte parts of row r at part ^ (r & 7)
-constexpr int kEpiWarpBytes = 3 * kPieceBytes;    // term, result, mirrored result
+constexpr int kEpiWarpBytes = 3 * kPieceBytes;    // term, result, mirrored result or a second term
 constexpr int kMaxStages = 4;
 
 template <int kCtas, int kPlanes>
@@ -80,7 +80,7 @@ struct alignas(8) Barriers {
     uint64_t empty[kMaxStages];
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
-    uint64_t term_full[kEpiWarps];
+    uint64_t term_full[2 * kEpiWarps];
     uint32_t tmem_base;
     uint32_t abort;
     uint32_t skip;
@@ -193,6 +193,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t sm
                  "r"(c0), "r"(c1), "r"(smem_src)
                  : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
@@ -202,20 +206,21 @@ template <int kPlanes, int kCols>
 struct Drain {
     const NsProduct *p;
     uint8_t *buffers;     // this warp's
-    uint64_t *term_full;  // this warp's barrier
-    uint32_t &term_phase;
+    uint64_t *term_full;  // this warp's two barriers
+    uint32_t &term_phase; // bit b: phase of barrier b
     int row0, col0, lane;
     int per_piece;        // loads of a piece: terms x planes
     bool mirror;
 
-    // load `index` of the tile: piece by piece, E before F, plane 0 before plane 1
-    __device__ __forceinline__ void fetch(int index) const
+    // Load r of a piece: E before F, plane 0 before plane 1.  Even ones go to the term buffer, odd ones to the mirror
+    // buffer, which must have been stored from by then.
+    __device__ __forceinline__ void fetch(int piece, int r) const
     {
-        if (lane != 0 || index >= per_piece * (kCols / kPieceCols)) return;
-        const int piece = index / per_piece, rest = index % per_piece;
-        mbar_expect_tx(term_full, kPieceBytes);
-        tma_load_2d<1>(buffers, &p->map_term[rest / kPlanes], col0 + piece * kPieceCols,
-                       row0 + (rest % kPlanes) * p->plane_rows, smem_u32(term_full));
+        if (lane != 0 || r >= per_piece || piece >= kCols / kPieceCols) return;
+        uint64_t *full = term_full + (r & 1);
+        mbar_expect_tx(full, kPieceBytes);
+        tma_load_2d<1>(buffers + (r & 1) * 2 * kPieceBytes, &p->map_term[r / kPlanes], col0 + piece * kPieceCols,
+                       row0 + (r % kPlanes) * p->plane_rows, smem_u32(full));
     }
     // one plane of a finished piece: h[k] holds columns 2k and 2k + 1 of this lane's row
     __device__ __forceinline__ void store(const uint32_t (&h)[32], int piece, int plane) const
@@ -253,9 +258,12 @@ struct Drain {
                                         Fn &&drained)
     {
         const float cg = p->g * mult;
-        int index = 0;  // of the load to wait for
 #pragma unroll 1
         for (int piece = 0; piece < kCols / kPieceCols; ++piece) {
+            if (piece > 0 && per_piece > 1) {
+                if (lane == 0) bulk_wait_read();
+                fetch(piece, 1);
+            }
             float f[kPieceCols];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -267,10 +275,11 @@ struct Drain {
             if (piece + 1 == kCols / kPieceCols) drained();
 #pragma unroll 1
             for (int r = 0; r < per_piece; ++r) {
-                if (!__all_sync(0xffffffffu, mbar_wait(term_full, term_phase, abort_flag, wait_limit))) return false;
-                term_phase ^= 1u;
+                const int buf = r & 1;
+                if (!__all_sync(0xffffffffu, mbar_wait(term_full + buf, (term_phase >> buf) & 1u, abort_flag, wait_limit))) return false;
+                term_phase ^= 1u << buf;
                 const float c = p->term[r / kPlanes] * mult;
-                const uint32_t row = smem_u32(buffers) + (uint32_t)(lane * 128);
+                const uint32_t row = smem_u32(buffers) + (uint32_t)(buf * 2 * kPieceBytes + lane * 128);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     uint32_t w[4];
@@ -283,7 +292,8 @@ struct Drain {
                     }
                 }
                 __syncwarp();
-                fetch(++index);
+                if (r + 2 < per_piece) fetch(piece, r + 2);
+                else if (buf == 0) fetch(piece + 1, 0);
             }
             uint32_t h[32];
 #pragma unroll
@@ -343,7 +353,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             mbar_init(&bars->tmem_full[a], 1);
             mbar_init(&bars->tmem_empty[a], kCtas * kEpiWarps);
         }
-        for (int w = 0; w < kEpiWarps; ++w) mbar_init(&bars->term_full[w], 1);
+        for (int w = 0; w < 2 * kEpiWarps; ++w) mbar_init(&bars->term_full[w], 1);
         bars->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -388,6 +398,10 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * 128;
             const int plane_rows = uniform(ti.p->plane_rows);
             const CUtensorMap *map_a = &ti.p->map_a, *map_b = &ti.p->map_b;
+            if (elected) {
+                prefetch_map(map_a);
+                prefetch_map(map_b);
+            }
             if (!__all_sync(0xffffffffu, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device, abort_flag,
                                                      wait_limit))) {
                 ok = false;
@@ -450,14 +464,21 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                     }
                     tcgen05_fence_after();
                     const uint32_t tmem_d = tmem + (uint32_t)(acc * C::BN);
+                    bool ready = false;
 #pragma unroll 1
                     for (int kb = k0; kb < k1; ++kb) {
-                        if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * stage, phase, abort_flag, wait_limit))) {
+                        if (!ready && !__all_sync(0xffffffffu, mbar_wait(full0 + 8 * stage, phase, abort_flag, wait_limit))) {
                             ok = false;
                             break;
                         }
                         tcgen05_fence_after();
-                        const uint32_t slot = (uint32_t)stage * (C::kStageBytes >> 4);
+                        const uint32_t slot = (uint32_t)stage * (C::kStageBytes >> 4), used = empty0 + 8 * stage;
+                        if (++stage == C::kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                        // a look at the next slot's barrier, answered while this one's products are issued
+                        const bool peek = kb + 1 < k1 && mbar_try_wait(full0 + 8 * stage, phase);
                         if (elected) {
                             // two planes: three products, smallest first; the dropped low x low is below 2^-22
 #pragma unroll
@@ -470,14 +491,10 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                                     tcgen05_mma_bf16<kCtas>(tmem_d, da + kk * (32 >> 4), db + kk * step_b, idesc,
                                                             (kb > k0 || term > 0 || kk > 0) ? 1u : 0u);
                             }
-                            tcgen05_commit<kCtas>(empty0 + 8 * stage);
+                            tcgen05_commit<kCtas>(used);
                             if (kb + 1 == k1) tcgen05_commit<kCtas>(&bars->tmem_full[acc]);
                         }
-                        __syncwarp();
-                        if (++stage == C::kStages) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
+                        ready = __all_sync(0xffffffffu, peek);
                     }
                     if (!ok) break;
                     acc ^= 1;
@@ -495,7 +512,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         constexpr int kCols = C::BN / 2;
         const int quarter = warp & 3, col_half = (warp - kFirstEpiWarp) >> 2;
         uint8_t *const my_buffers = epi_stage + (size_t)(warp - kFirstEpiWarp) * kEpiWarpBytes;
-        uint64_t *const term_full = &bars->term_full[warp - kFirstEpiWarp];
+        uint64_t *const term_full = &bars->term_full[2 * (warp - kFirstEpiWarp)];
         uint32_t term_phase = 0;
         int acc = 0;
         uint32_t acc_phase = 0;
@@ -516,6 +533,10 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             // extents are multiples of 128: a warp's share is all in or all out
             const bool inside = row0 < p->M && col0 < p->N;
             Drain<kPlanes, kCols> drain{p, my_buffers, term_full, term_phase, row0, col0, lane, p->n_terms * kPlanes, ti.mirror};
+            if (lane == 0) {
+                if (p->n_terms > 0) prefetch_map(&p->map_term[0]);
+                prefetch_map(&p->map_d);
+            }
             if (inside && drain.per_piece > 0) {  // the first term: its matrix must be stored
                 if (!__all_sync(0xffffffffu, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device,
                                                          abort_flag, wait_limit))) {
@@ -523,7 +544,8 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                     break;
                 }
                 asm volatile("fence.proxy.async;" ::: "memory");
-                drain.fetch(0);
+                drain.fetch(0, 0);
+                drain.fetch(0, 1);
             }
             auto drained = [&](int buffer) {
                 tcgen05_fence_before();
@@ -602,7 +624,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         for (int s = 0; s < C::kStages; ++s)
             for (uint32_t i = 0; i < 4096u; ++i)
                 if (mbar_try_wait(&bars->full[s], 0) || mbar_try_wait(&bars->full[s], 1)) break;
-        for (int w = 0; w < kEpiWarps; ++w)
+        for (int w = 0; w < 2 * kEpiWarps; ++w)
             for (uint32_t i = 0; i < 4096u; ++i)
                 if (mbar_try_wait(&bars->term_full[w], 0) || mbar_try_wait(&bars->term_full[w], 1)) break;
     }
