@@ -8,7 +8,7 @@
 //
 // X (n x m) is cut by columns over the cluster; a CTA's share is read once for the norm, once more (from L2) to
 // be scaled by a power of two into f16 planes in shared memory, and stays there: 64 columns are an 8 KiB block
-// that serves as K-major operand of the Gram and as MN-major operand of the update alike.  The Gram's
+// that serves, along one direction or the other, as operand of the Gram and of the update alike.  The Gram's
 // partial sums are added over the cluster through distributed shared memory in rank order, so all CTAs hold the
 // same bits and run the same short-side program, the planner's products (ns_plan.cu), with all of its matrices
 // in shared memory as two f16 planes.  With 22 bits on the short side the groups of steps can be long: in
@@ -59,11 +59,11 @@ __device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float
 
 // f += c * (16 values of one row of a block, columns col .. col + 15, all planes)
 template <int kPlanes>
-__device__ __forceinline__ void add_row(float (&f)[kCols], float c, uint32_t block, int row, int col)
+__device__ __forceinline__ void add_row(float (&f)[kCols], float c, uint32_t block, uint32_t plane, int row, int col)
 {
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl) {
-        const uint32_t at = block + (uint32_t)(pl * kBlockBytes + row * 128);
+        const uint32_t at = block + pl * plane + (uint32_t)(row * 128);
 #pragma unroll
         for (int q = 0; q < kCols / 8; ++q) {
             uint32_t v[4];
@@ -78,11 +78,11 @@ __device__ __forceinline__ void add_row(float (&f)[kCols], float c, uint32_t blo
     }
 }
 template <int kPlanes>
-__device__ __forceinline__ void put_row(float (&f)[kCols], uint32_t block, int row, int col)
+__device__ __forceinline__ void put_row(float (&f)[kCols], uint32_t block, uint32_t plane, int row, int col)
 {
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl) {
-        const uint32_t at = block + (uint32_t)(pl * kBlockBytes + row * 128);
+        const uint32_t at = block + pl * plane + (uint32_t)(row * 128);
 #pragma unroll
         for (int q = 0; q < kCols / 8; ++q) {
             uint32_t h[4];
@@ -100,18 +100,23 @@ __device__ __forceinline__ void put_row(float (&f)[kCols], uint32_t block, int r
     }
 }
 
-// A (128 x 64, rows from 64 on unused) times B (64 x 64) into 64 accumulator columns; operands are blocks of
-// kA and kB planes, the products of their planes smallest first.  `a` and `b` are descriptors of plane 0 (see
-// Descriptors): other planes and k slices are reached by adding to the address field.  k_slices: 16 each.  The whole
-// warp runs this, its elected lane issues.
+// An operand of M (or N) x 64: the descriptor of its plane 0, what to add to its address field for the next plane
+// and for the next 16 of the contraction, and which way it lies.
+struct Operand {
+    uint64_t desc;
+    uint32_t plane, step;
+    bool mn_major;
+};
+// A (M = 128) times B (N = 64) into 64 accumulator columns, the products of their planes smallest first.  The whole
+// warp runs this, its elected lane issues.  k_slices: 16 each.
 template <int kA, int kB>
-__device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_t b, bool b_mn, bool accumulate, int k_slices,
+__device__ __forceinline__ void issue_product(uint32_t tmem, const Operand &a, const Operand &b, bool accumulate, int k_slices,
                                               bool elected)
 {
-    // f32 accumulator, f16 operands, A K-major, M = 128, N = 64
-    const uint32_t idesc = (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(kSide >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-    const uint32_t step_b = b_mn ? 2048 >> 4 : 32 >> 4;
-    uint32_t keep = accumulate ? 1u : 0u;
+    // f32 accumulator, f16 operands, M = 128, N = 64
+    const uint32_t idesc = (1u << 4) | ((uint32_t)a.mn_major << 15) | ((uint32_t)b.mn_major << 16) |
+                           ((uint32_t)(kSide >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    bool first = true;
 #pragma unroll
     for (int t = kA + kB - 2; t >= 0; --t) {  // plane of A + plane of B; low x low is dropped
         if (kA == 2 && kB == 2 && t == 2) continue;
@@ -119,13 +124,13 @@ __device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_
         for (int pa = 0; pa < kA; ++pa) {
             const int pb = t - pa;
             if (pb < 0 || pb >= kB) continue;
-#pragma unroll 1
-            for (int kk = 0; kk < k_slices; ++kk) {
-                if (elected)
-                    tcgen05_mma_bf16<1>(tmem, a + (uint32_t)(pa * (kBlockBytes >> 4) + kk * (32 >> 4)),
-                                        b + (uint32_t)(pb * (kBlockBytes >> 4)) + kk * step_b, idesc, keep);
-                keep = 1u;
+#pragma unroll
+            for (int kk = 0; kk < kSide / 16; ++kk) {
+                if (elected && kk < k_slices)
+                    tcgen05_mma_bf16<1>(tmem, a.desc + pa * a.plane + kk * a.step, b.desc + pb * b.plane + kk * b.step, idesc,
+                                        (first && kk == 0) ? (accumulate ? 1u : 0u) : 1u);
             }
+            first = false;
         }
     }
 }
@@ -133,8 +138,11 @@ __device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_
 struct Descriptors {
     uint64_t k_major, mn_major;  // of address 0
     __device__ __forceinline__ Descriptors() : k_major(make_smem_desc(0, 16, 1024)), mn_major(make_smem_desc(0, kBlockBytes, 1024)) {}
-    __device__ __forceinline__ uint64_t rows(uint32_t addr) const { return k_major + (addr >> 4); }
-    __device__ __forceinline__ uint64_t columns(uint32_t addr) const { return mn_major + (addr >> 4); }
+    // `addr` holds rows of 64 along the contraction, or 64 rows of the contraction
+    __device__ __forceinline__ Operand operand(uint32_t addr, uint32_t plane, bool mn) const
+    {
+        return {(mn ? mn_major : k_major) + (addr >> 4), plane >> 4, mn ? 2048u >> 4 : 32u >> 4, mn};
+    }
 };
 __device__ __forceinline__ void tmem_ld_16_sync(uint32_t taddr, float (&f)[kCols])
 {
@@ -280,26 +288,18 @@ __device__ __forceinline__ void for_u(const NsElementwise &w, const NsMatrixArg 
     }
 }
 
-// h[e] <- h[(e + turn) mod 8], turn in 0 .. 8
-__device__ __forceinline__ void rotate8(__half (&h)[8], int turn)
-{
-#pragma unroll
-    for (int bit = 1; bit < 8; bit *= 2) {
-        const bool move = (turn & bit) != 0;
-        __half r[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = move ? h[(e + bit) & 7] : h[e];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = r[e];
+// X in shared memory: plane p's block b (64 columns of X) at (p blocks + b) 8 KiB, as 64 rows of 128 bytes; a row is
+// a row of X, or (turned) a column.
+struct Image {
+    uint32_t base, plane;
+    bool turned;
+    __device__ __forceinline__ uint32_t block(int b) const { return base + (uint32_t)(b * kBlockBytes); }
+    __device__ __forceinline__ uint32_t at(int i, int j) const
+    {
+        const int r = turned ? j & 63 : i, c = turned ? i : j & 63;
+        return block(j >> 6) + (uint32_t)(r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
     }
-}
-
-// Where element (i, j) of X lies in shared memory (plane 0)
-template <int kPlanes>
-__device__ __forceinline__ uint32_t x_address(uint32_t x_base, int i, int j)
-{
-    return x_base + (uint32_t)((j >> 6) * kPlanes * kBlockBytes + i * 128 + ((((j & 63) >> 3) ^ (i & 7)) << 4) + (j & 7) * 2);
-}
+};
 
 __device__ __forceinline__ void report(const NsError &error)
 {
@@ -318,7 +318,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     uint8_t *x_bytes = smem + kSquaresBytes;
     const int blocks = small.columns / 64;
     Shared &sh = *reinterpret_cast<Shared *>(x_bytes + (size_t)blocks * kPlanes * kBlockBytes + kBlockBytes);
-    const uint32_t squares = smem_u32(smem), x_base = smem_u32(x_bytes);
+    const uint32_t squares = smem_u32(smem);
 
     const int clusters = small.cluster, rank = (int)blockIdx.x % clusters;
     const int index = (int)blockIdx.x / clusters;
@@ -341,6 +341,9 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+
+    // X lies in shared memory as the first array lies in memory: whole 16-byte pieces move, no transposition
+    const Image x{smem_u32(x_bytes), (uint32_t)(blocks * kBlockBytes), walks_i(a.a[kStep ? 1 : 0])};
 
     // ---- the norm: every CTA of the cluster its columns, then all sums in rank order ----
     const Share s{d.n, d.m, rank * small.columns, small.columns, walks_i(a.a[kStep ? 1 : 0])};
@@ -377,28 +380,14 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         __half h[8], l[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = e < count ? u[e] * up0 * up1 : 0.0f;
-            h[e] = __float2half_rn(x);
-            l[e] = __float2half_rn(x - __half2float(h[e]));
+            const float z = e < count ? u[e] * up0 * up1 : 0.0f;
+            h[e] = __float2half_rn(z);
+            l[e] = __float2half_rn(z - __half2float(h[e]));
         }
-        if (s.along_i) {
-            // lanes of a warp hold different groups of 8 rows and the same few columns: in step e a lane stores its
-            // row (e + group) mod 8, so that their 16-byte parts, which the swizzle places by row mod 8, differ
-            const int turn = (i >> 3) & 7;
-            rotate8(h, turn);
-            if (kPlanes == 2) rotate8(l, turn);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t at = x_address<kPlanes>(x_base, i + ((e + turn) & 7), j);
-                asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(h[e])) : "memory");
-                if (kPlanes == 2) asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + kBlockBytes), "h"(__half_as_ushort(l[e])) : "memory");
-            }
-        } else {
-            const uint32_t at = x_address<kPlanes>(x_base, i, j);
-            const uint4 qh = *reinterpret_cast<const uint4 *>(h), ql = *reinterpret_cast<const uint4 *>(l);
-            st_shared_128(at, qh.x, qh.y, qh.z, qh.w);
-            if (kPlanes == 2) st_shared_128(at + kBlockBytes, ql.x, ql.y, ql.z, ql.w);
-        }
+        const uint32_t at = x.at(i, j);  // along the image's rows: s.along_i == x.turned
+        const uint4 qh = *reinterpret_cast<const uint4 *>(h), ql = *reinterpret_cast<const uint4 *>(l);
+        st_shared_128(at, qh.x, qh.y, qh.z, qh.w);
+        if (kPlanes == 2) st_shared_128(at + x.plane, ql.x, ql.y, ql.z, ql.w);
     });
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
@@ -428,6 +417,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         tcgen05_fence_after();
     };
     auto square = [&](int k) { return squares + (uint32_t)(k * kSquareBytes); };
+    auto square_operand = [&](int k) { return desc.operand(square(k), kBlockBytes, false); };
 
     for (int op0 = 0; op0 < d.n_ops;) {
         const NsSmallOp first = sh.ops[op0];
@@ -441,8 +431,8 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             for (int b0 = 0; b0 < blocks; b0 += chunk) {
                 if (issuer && !dead && !withhold) {
                     for (int k = b0; k < min(b0 + chunk, blocks); ++k) {
-                        const uint64_t x = desc.rows(x_base + (uint32_t)(k * kPlanes * kBlockBytes));
-                        issue_product<kPlanes, kPlanes>(tmem, x, x, false, k > b0, kSide / 16, elected);
+                        const Operand o = desc.operand(x.block(k), x.plane, x.turned);  // turned: columns of X are rows
+                        issue_product<kPlanes, kPlanes>(tmem, o, o, k > b0, kSide / 16, elected);
                     }
                     if (elected) tcgen05_commit<1>(&sh.done);
                 }
@@ -497,7 +487,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 const float c = first.g * (first.scale_power == 2 ? scale * scale : 1.0f);
 #pragma unroll
                 for (int k = 0; k < kCols; ++k) g[k] *= c;
-                put_row<2>(g, square(first.D), row, col);
+                put_row<2>(g, square(first.D), kBlockBytes, row, col);
             }
             release();
             op0 += 1;
@@ -506,8 +496,8 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             const int count = first.stage_ops;
             if (issuer && !dead) {
                 for (int k = 0; k < count; ++k)
-                    issue_product<2, 2>(tmem + (uint32_t)(k * 64), desc.rows(square(uniform((int)sh.ops[op0 + k].A))),
-                                        desc.rows(square(uniform((int)sh.ops[op0 + k].B))), false, false, k_slices, elected);
+                    issue_product<2, 2>(tmem + (uint32_t)(k * 64), square_operand(uniform((int)sh.ops[op0 + k].A)),
+                                        square_operand(uniform((int)sh.ops[op0 + k].B)), false, k_slices, elected);
                 if (elected) tcgen05_commit<1>(&sh.done);
             }
             // the terms that are there already, while the products run
@@ -519,8 +509,8 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                     for (int j = 0; j < kCols; ++j) f[k][j] = 0.0f;
                     if (k >= count) continue;
                     const NsSmallOp op = sh.ops[op0 + k];
-                    if (op.E >= 0) add_row<2>(f[k], op.e, square(op.E), row, col);
-                    if (op.F >= 0) add_row<2>(f[k], op.f, square(op.F), row, col);
+                    if (op.E >= 0) add_row<2>(f[k], op.e, square(op.E), kBlockBytes, row, col);
+                    if (op.F >= 0) add_row<2>(f[k], op.f, square(op.F), kBlockBytes, row, col);
                 }
             }
             wait_done();
@@ -533,33 +523,40 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                     const float c = sh.ops[op0 + k].g;
 #pragma unroll
                     for (int j = 0; j < kCols; ++j) f[k][j] = fmaf(c, v[j], f[k][j]);
-                    put_row<2>(f[k], square(sh.ops[op0 + k].D), row, col);
+                    put_row<2>(f[k], square(sh.ops[op0 + k].D), kBlockBytes, row, col);
                 }
             }
             release();
             op0 += count;
         } else {
-            // ---- update of X, four blocks of 64 columns at a time, in place ----
+            // ---- update of X in place, 256 accumulator columns at a time ----
+            // P X for four blocks (X's rows in 64 lanes), or, turned, X^T P (P is symmetric) for eight: two blocks
+            // follow each other in memory as the 128 rows of one operand
             const float mult = first.scale_power == 1 ? scale : 1.0f;
             const float ce = first.e * mult, cg = first.g * mult;
-            for (int b0 = 0; b0 < blocks; b0 += 4) {
-                const int b1 = min(b0 + 4, blocks);
+            const int per_product = x.turned ? 2 : 1;
+            const Operand P = square_operand(uniform((int)first.A));
+            for (int b0 = 0; b0 < blocks; b0 += 4 * per_product) {
+                const int products = min(4, (blocks - b0 + per_product - 1) / per_product);
                 if (issuer && !dead) {
-                    for (int k = b0; k < b1; ++k)
-                        issue_product<2, kPlanes>(tmem + (uint32_t)((k - b0) * 64), desc.rows(square(uniform((int)first.A))),
-                                                  desc.columns(x_base + (uint32_t)(k * kPlanes * kBlockBytes)), true, false, k_slices, elected);
+                    for (int k = 0; k < products; ++k) {
+                        const Operand X = desc.operand(x.block(b0 + k * per_product), x.plane, !x.turned);
+                        if (x.turned) issue_product<kPlanes, 2>(tmem + (uint32_t)(k * 64), X, P, false, k_slices, elected);
+                        else issue_product<2, kPlanes>(tmem + (uint32_t)(k * 64), P, X, false, k_slices, elected);
+                    }
                     if (elected) tcgen05_commit<1>(&sh.done);
                 }
                 wait_done();
-                if (worker) {
-                    for (int k = b0; k < b1; ++k) {
-                        const uint32_t block = x_base + (uint32_t)(k * kPlanes * kBlockBytes);
+                if (worker || x.turned) {
+                    for (int k = 0; k < products; ++k) {
+                        const int at = b0 + k * per_product + (row >> 6);
                         float f[kCols];
-                        tmem_ld_16_sync(my_tmem + (uint32_t)((k - b0) * 64), f);
+                        tmem_ld_16_sync(my_tmem + (uint32_t)(k * 64), f);  // the whole warp
+                        if (at >= blocks) continue;
 #pragma unroll
                         for (int j = 0; j < kCols; ++j) f[j] *= cg;
-                        add_row<kPlanes>(f, ce, block, row, col);
-                        put_row<kPlanes>(f, block, row, col);
+                        add_row<kPlanes>(f, ce, x.block(at), x.plane, row & 63, col);
+                        put_row<kPlanes>(f, x.block(at), x.plane, row & 63, col);
                     }
                 }
                 release();
@@ -595,28 +592,21 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 for (int e = 0; e < 8; ++e) f[e] = 0.0f;
 #pragma unroll
                 for (int pl = 0; pl < kPlanes; ++pl) {
-                    if (out.along_i) {  // as the stores above, the other way round
-                        const int turn = (i >> 3) & 7;
-                        __half h[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            unsigned short x;
-                            asm volatile("ld.shared.b16 %0, [%1];"
-                                         : "=h"(x)
-                                         : "r"(x_address<kPlanes>(x_base, i + ((e + turn) & 7), j) + pl * kBlockBytes)
-                                         : "memory");
-                            h[e] = __ushort_as_half(x);
-                        }
-                        rotate8(h, 8 - turn);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] += __half2float(h[e]);
-                    } else {
+                    if (out.along_i == x.turned) {
                         uint32_t v[4];
-                        ld_shared_128(x_address<kPlanes>(x_base, i, j) + pl * kBlockBytes, v[0], v[1], v[2], v[3]);
+                        ld_shared_128(x.at(i, j) + pl * x.plane, v[0], v[1], v[2], v[3]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float2 x = unpack_half(v[e]);
-                            f[2 * e] += x.x, f[2 * e + 1] += x.y;
+                            const float2 z = unpack_half(v[e]);
+                            f[2 * e] += z.x, f[2 * e + 1] += z.y;
+                        }
+                    } else {  // the caller's array lies the other way
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            unsigned short h;
+                            const uint32_t from = out.along_i ? x.at(i + e, j) : x.at(i, j + e);
+                            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(from + pl * x.plane) : "memory");
+                            f[e] += __half2float(__ushort_as_half(h));
                         }
                     }
                 }
