@@ -64,6 +64,50 @@ __device__ __forceinline__ void store8(int type, void *base, int64_t at, int64_t
     else store8_as(static_cast<__half *>(base) + at, step, count, vec, v);
 }
 
+__device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+
+// 8 elements as they lie in memory (whole and aligned octets; others are read when they are asked for): loads first,
+// conversions later, so that a thread has several octets on their way.
+struct Raw {
+    uint4 q[2];
+    bool packed;
+    __device__ __forceinline__ void load(int type, const void *base, int64_t at, int count, bool vec)
+    {
+        packed = vec && count == 8;
+        if (packed) {
+            const char *p = static_cast<const char *>(base) + at * (type == VB_DTYPE_F32 ? 4 : 2);
+            q[0] = *reinterpret_cast<const uint4 *>(p);
+            if (type == VB_DTYPE_F32) q[1] = reinterpret_cast<const uint4 *>(p)[1];
+        }
+    }
+    __device__ __forceinline__ void get(int type, const void *base, int64_t at, int64_t step, int count, float (&v)[8]) const
+    {
+        if (!packed) {
+            load8(type, base, at, step, count, false, v);
+            return;
+        }
+        if (type == VB_DTYPE_F32) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                v[4 * k] = __uint_as_float(q[k].x), v[4 * k + 1] = __uint_as_float(q[k].y);
+                v[4 * k + 2] = __uint_as_float(q[k].z), v[4 * k + 3] = __uint_as_float(q[k].w);
+            }
+        } else {
+            const uint32_t h[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (type == VB_DTYPE_BF16) {
+                    v[2 * k] = __uint_as_float(h[k] << 16);
+                    v[2 * k + 1] = __uint_as_float(h[k] & 0xffff0000u);
+                } else {
+                    const float2 x = unpack_half(h[k]);
+                    v[2 * k] = x.x, v[2 * k + 1] = x.y;
+                }
+            }
+        }
+    }
+};
+
 // along i where that is the contiguous direction and j is not
 __device__ __forceinline__ bool walks_i(const NsArray &a) { return a.si == 1 && a.sj != 1; }
 // U of one octet in the velocity's direction: new velocity in v, U in u.

@@ -38,8 +38,10 @@ constexpr int kMaxSteps = 64;
 constexpr int64_t kMaxSide = 65536;
 constexpr uint32_t kDefaultWaitLimit = 1u << 22;  // polls, about a second
 constexpr double kDiverged = 1048576.0;
-// norm and gather of a batch follow each other; a batch's arrays should stay in the 126 MB L2 in between
-constexpr int64_t kBatchElements = 8 << 20;
+// Elements of an element-wise launch.  Norm and gather of a batch follow each other; small batches would find the
+// second read in the L2 cache, but their launches fill and drain more often: 4, 8, 16, 64 Mi elements measured
+// 1073, 970, 886, 748 us for the d = 1024 set.
+constexpr int64_t kBatchElements = 64 << 20;
 
 // ---- schedule ----------------------------------------------------------------------------
 enum BufferId { BUF_X0 = 0, BUF_X1 = 1, BUF_SQUARE = 2 };  // BUF_SQUARE + k: k-th short-side matrix
@@ -264,6 +266,7 @@ struct vb_ns_matrices {
     std::vector<vb::NsArray> arrays;  // in the working orientation
     std::vector<uint8_t> vec;         // rows (or columns) on 16-byte boundaries
     bool writable = true;             // no two elements at one address
+    bool turned = false;              // an array is contiguous along the short side
     bool any_null = false;            // a matrix with elements has no array
     const char *why = "";             // why it is not writable
 };
@@ -347,6 +350,16 @@ uint32_t for_tiles(const NsProduct &pr, int shape, Fn &&fn)
     for (int m0 = 0; m0 < pr.M; m0 += bm)
         for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn, ++count) fn(m0, n0, symmetric && n0 > m0);
     return count;
+}
+
+// Into how many pieces the contraction of a product is cut: a Gram over a long side whose stage would leave most
+// SMs idle (128 x 9216: one tile of 144 blocks) is spread over them, in pieces of at least 8 blocks.  Summing the
+// pieces is a stage more, about 8 us: a block takes 0.4 us (0.6 with two planes), so 32 blocks are where it pays
+// (at 16, 513 x 1000, it cost 28 us of 158).
+int gram_parts(const NsProduct &pr, int shape, uint32_t stage_tiles, int sm_count)
+{
+    if (shape != NS_TILE_128 || (pr.flags & NS_GRAM) == 0 || stage_tiles == 0 || pr.K < 32 * kNsKBlock) return 1;
+    return std::max(1, std::min(pr.K / kNsKBlock / 8, sm_count / (int)stage_tiles));
 }
 
 // The shape whose stages take less time if every stage is waited for: whole rounds of tiles over the
@@ -480,9 +493,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         p->ew.stored = c.take<uint32_t>((size_t)n);
         p->error.device = c.take<uint32_t>(1);
         p->ew.error = p->error.device;
-        NsMatrixDims *d_dims = c.take<NsMatrixDims>((size_t)n);
         int32_t *d_tile_matrix = c.take<int32_t>(tile_matrix.size());
-        p->ew.dims = d_dims;
         NsSmallMatrix *d_small = c.take<NsSmallMatrix>(small.size());
         NsSmallOp *d_small_ops = c.take<NsSmallOp>(small_ops.size());
         p->small.matrices = d_small;
@@ -514,7 +525,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                     q.scale_power = pr.scale_power;
                     q.scale = p->ew.scale + i;
                     q.matrix = (int32_t)i;
-                    q.flags = pr.update ? NS_B_MN_MAJOR : 0;
+                    q.flags = (pr.update ? NS_B_MN_MAJOR : 0) | (pr.gram ? NS_GRAM : 0);
                     if (round == 1) {
                         const int64_t outer = (int64_t)p->planes * d.np;
                         VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, outer, NS_MAP_ROWS));
@@ -536,22 +547,60 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         tile_list.clear();
         std::vector<uint32_t> done((size_t)n, 0), stage_done((size_t)n, 0);
         size_t widest = 0;
+        auto count_tiles = [&](const NsProduct &pr) { return for_tiles(pr, p->shape, [](int, int, bool) {}); };
+        std::vector<uint32_t> stage_tiles(n_stages, 0);
+        for (size_t k = 0; k < n_stages; ++k)
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) stage_tiles[k] += count_tiles(problems[q]);
+        // every matrix has slots of its own for the pieces of its Grams, which follow one another
+        std::vector<int32_t> slot0((size_t)n, 0);
+        for (size_t k = 0; k < n_stages; ++k)
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
+                const int parts = gram_parts(problems[q], p->shape, stage_tiles[k], p->eng->sm_count);
+                int32_t &need = slot0[(size_t)problems[q].matrix];
+                if (parts > 1) need = std::max(need, (int32_t)count_tiles(problems[q]) * parts);
+            }
+        int32_t slots = 0;
+        for (int32_t &s : slot0) {
+            const int32_t need = s;
+            s = slots;
+            slots += need;
+        }
         for (size_t k = 0; k < n_stages; ++k) {
             const size_t stage_at = tile_list.size();
+            std::vector<NsTile> sums;  // of cut contractions, behind the stage's other tiles
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
-                const size_t i = (size_t)problems[q].matrix;
-                stage_done[i] += for_tiles(problems[q], p->shape, [&](int m0, int n0, bool mirror) {
-                    tile_list.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, done[i], 0});
+                const NsProduct &pr = problems[q];
+                const size_t i = (size_t)pr.matrix;
+                const int blocks = pr.K / kNsKBlock;
+                const int parts = gram_parts(pr, p->shape, stage_tiles[k], p->eng->sm_count);
+                int32_t slot = slot0[i];
+                uint32_t count = 0;
+                for_tiles(pr, p->shape, [&](int m0, int n0, bool mirror) {
+                    if (parts == 1) {
+                        tile_list.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, done[i], 0, blocks, -1, 0});
+                        ++count;
+                        return;
+                    }
+                    sums.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, 0, 0, 0, slot, parts});
+                    for (int part = 0; part < parts; ++part, ++count)
+                        tile_list.push_back({(int32_t)q, m0, n0, 0, done[i], blocks * part / parts, blocks * (part + 1) / parts, slot++, 0});
                 });
+                stage_done[i] += count;
             }
             widest = std::max(widest, tile_list.size() - stage_at);
+            for (NsTile &t : sums) t.after = stage_done[(size_t)problems[(size_t)t.problem].matrix];
+            for (const NsTile &t : sums) {
+                tile_list.push_back(t);
+                stage_done[(size_t)problems[(size_t)t.problem].matrix] += 1;
+            }
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) done[(size_t)problems[q].matrix] = stage_done[(size_t)problems[q].matrix];
         }
+        float *partials = c.take<float>((size_t)slots * 128 * 128);
         NsProduct *d_problems = c.take<NsProduct>(problems.size());
         NsTile *d_tiles = c.take<NsTile>(tile_list.size());
         if (tile_list.size() > (size_t)INT32_MAX) return fail(VB_ERR_UNSUPPORTED, "the plan's products have too many tiles");
         // more CTAs (pairs) than the largest stage has tiles would mostly wait, on SMs that others could use
-        p->products = {d_problems, d_tiles, p->ew.stored, (int)tile_list.size(), (int)widest};
+        p->products = {d_problems, d_tiles, p->ew.stored, partials, (int)tile_list.size(), (int)widest};
         if (round == 1) {
             VB_CUDA(cudaMemcpyAsync(d_problems, problems.data(), problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
@@ -564,7 +613,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             // wait for a whole stage
             p->default_wait_limit = (uint32_t)std::min(1e9, kDefaultWaitLimit * (1.0 + 2.0 * std::floor(stage_flops / 1e14)));
             for (const NsTile &t : tile_list)
-                p->flops += 2.0 * (p->planes == 2 ? 3.0 : 1.0) * bm * bn * problems[(size_t)t.problem].K;
+                p->flops += 2.0 * (p->planes == 2 ? 3.0 : 1.0) * bm * bn * (double)(t.kb1 - t.kb0) * kNsKBlock;
         }
         if (round == 0) {
             p->workspace = c.used;
@@ -575,7 +624,6 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                 VB_CUDA(cudaMemcpyAsync(d_small_ops, small_ops.data(), small_ops.size() * sizeof(NsSmallOp), cudaMemcpyHostToDevice, p->eng->stream));
             }
             VB_CUDA(cudaMemsetAsync(p->error.device, 0, sizeof(uint32_t), p->eng->stream));
-            VB_CUDA(cudaMemcpyAsync(d_dims, p->dims.data(), (size_t)n * sizeof(NsMatrixDims), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tile_matrix, tile_matrix.data(), tile_matrix.size() * sizeof(int32_t), cudaMemcpyHostToDevice, p->eng->stream));
         }
     }
@@ -593,7 +641,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
 
 // What both operators share; `fill` sets the arrays of one matrix.
 template <typename Fill>
-int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
+int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, bool turned, Fill &&fill)
 {
     vb_engine *e = p->eng;
     NsBatchArgs &args = *p->args;
@@ -602,7 +650,10 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
         args.count = b.count;
         args.tile0 = b.tile0;
         args.n_tiles = b.n_tiles;
-        for (int32_t k = 0; k < b.count; ++k) fill(b.first + k, args.m[k]);
+        for (int32_t k = 0; k < b.count; ++k) {
+            fill(b.first + k, args.m[k]);
+            args.m[k].d = p->dims[(size_t)(b.first + k)];
+        }
     };
     const uint32_t wait_limit = p->wait_limit ? p->wait_limit : p->default_wait_limit;
     cudaStream_t side = e->stream;
@@ -626,8 +677,8 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
     for (const auto &b : p->batches) {
         if (b.n_tiles == 0) continue;
         load(b);
-        VB_TRY(launch_ns_norm(w, args, p->d_tile_matrix, step, e->stream));
-        VB_TRY(launch_ns_gather(w, args, p->d_tile_matrix, step, e->stream));
+        VB_TRY(launch_ns_norm(w, args, p->d_tile_matrix, step, turned, e->stream));
+        VB_TRY(launch_ns_gather(w, args, p->d_tile_matrix, step, turned, e->stream));
         e->launches += 2;
     }
     prof_end(e, VB_PHASE_MUON_PRE);
@@ -643,7 +694,7 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, Fill &&fill)
     for (const auto &b : p->batches) {
         if (b.n_tiles == 0) continue;
         load(b);
-        VB_TRY(launch_ns_finish(w, args, p->d_tile_matrix, step, e->stream));
+        VB_TRY(launch_ns_finish(w, args, p->d_tile_matrix, step, turned, e->stream));
         e->launches += 1;
     }
     prof_end(e, VB_PHASE_MUON_APPLY);
@@ -844,6 +895,7 @@ int vb_ns_matrices_create(vb_ns_plan *p, int dtype, void *const *pointers, const
         if (m == 1) a.si = per16, a.sj = 1;
         const int64_t across = a.sj == 1 ? a.si : a.si == 1 ? a.sj : 1;
         l->vec[(size_t)i] = (a.sj == 1 || a.si == 1) && at % 16 == 0 && across % per16 == 0;
+        if (a.si == 1 && a.sj != 1) l->turned = true;
         const bool apart = (a.sj >= 1 && a.si >= (m - 1) * a.sj + 1) || (a.si >= 1 && a.sj >= (n - 1) * a.si + 1) ||
                            (n == 1 && (a.sj >= 1 || m == 1));
         if (!apart) l->writable = false, l->why = "elements of a matrix share an address";
@@ -875,7 +927,7 @@ int vb_orthogonalize(vb_ns_plan *p, const vb_ns_matrices *inputs, const vb_ns_ma
     w.eps = p->eps;
     w.types[0] = inputs->dtype;
     w.types[1] = outputs->dtype;
-    return run_plan(p, w, false, [&](int64_t i, NsMatrixArg &a) {
+    return run_plan(p, w, false, inputs->turned || outputs->turned, [&](int64_t i, NsMatrixArg &a) {
         const size_t k = (size_t)i;
         a.a[0] = inputs->arrays[k];
         a.a[1] = outputs->arrays[k];
@@ -911,7 +963,7 @@ int vb_muon_multi_tensor_step(vb_ns_plan *p, const vb_muon_step_params *hp, cons
     w.nesterov = hp->nesterov != 0;
     w.decay = (float)(1.0 - (double)hp->lr * (double)hp->weight_decay);
     w.rate = hp->lr;
-    return run_plan(p, w, true, [&](int64_t i, NsMatrixArg &a) {
+    return run_plan(p, w, true, grads->turned || velocities->turned || params->turned, [&](int64_t i, NsMatrixArg &a) {
         const size_t k = (size_t)i;
         a.a[0] = grads->arrays[k];
         a.a[1] = velocities->arrays[k];

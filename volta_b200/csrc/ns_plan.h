@@ -15,12 +15,14 @@
 
 namespace vb {
 
+constexpr int kNsKBlock = 64;  // of the contraction, as staged in shared memory
 constexpr int kNsPad = 128;  // sides of the working matrices are multiples of this
 
 // One product of the iteration:  D = e E + f F + g sum_k A[m,k] B[n,k]
 // E and F (f16, leading dimension and planes of D; may be null) are read at D's position.
 enum NsProductFlags {
     NS_B_MN_MAJOR = 1,  // B is stored [k][n] (the working matrix X); otherwise [n][k]
+    NS_GRAM = 2         // X X^T: the contraction runs over the long side
 };
 struct alignas(128) NsProduct {
     // tensor maps, see make_ns_map
@@ -42,7 +44,10 @@ struct NsTile {
     int32_t problem, m0, n0;
     int32_t mirror;   // symmetric product: the tile is also stored transposed
     uint32_t after;   // tiles of the matrix's earlier stages: all of them must be stored before this one starts
-    int32_t pad;
+    int32_t kb0, kb1; // blocks of 64 of the contraction
+    // A contraction cut into pieces (128 x 128 tiles): a piece (part >= 0, parts == 0) stores its f32 accumulator in
+    // slot `part`; the tile after them (parts > 0, no contraction of its own) sums slots part .. part + parts - 1 in order.
+    int32_t part, parts;
 };
 
 // The tiles of every stage of every matrix, earlier stages first.
@@ -50,6 +55,7 @@ struct NsLaunch {
     const NsProduct *problems;
     const NsTile *tiles;
     uint32_t *stored;  // per matrix: epilogue warps' arrivals, zeroed by the gather pass
+    float *partials;   // slots of 128 x 128
     int n_tiles;
     int widest;        // tiles of the largest stage
 };
@@ -84,12 +90,6 @@ struct NsArray {
     int64_t si, sj;
 };
 constexpr int kNsBatch = 96;  // matrices of one element-wise launch (bounded by its parameter space)
-struct NsMatrixArg {
-    NsArray a[3];   // orthogonalize: input, output; step: gradient, velocity, parameter
-    float scale;    // step: s_i of the update
-    uint32_t live;  // 0: no gradient, the matrix is left alone
-    uint32_t direct; // bit k: array k has sj == 1 and rows on 16-byte boundaries
-};
 struct NsMatrixDims {
     int32_t n, m;            // extents
     int32_t np, mp;          // padded
@@ -98,8 +98,14 @@ struct NsMatrixDims {
     float final_scale;       // a stored value of the last iterate times this is the value
     int32_t tile0, n_tiles;  // element-wise tiles of this matrix
 };
+struct NsMatrixArg {
+    NsArray a[3];   // orthogonalize: input, output; step: gradient, velocity, parameter
+    NsMatrixDims d;
+    float scale;    // step: s_i of the update
+    uint32_t live;  // 0: no gradient, the matrix is left alone
+    uint32_t direct; // bit k: array k has sj == 1 and rows on 16-byte boundaries
+};
 struct NsElementwise {
-    const NsMatrixDims *dims;  // of every matrix of the plan
     double *partials;          // one sum of squares per tile
     float *scale;              // per matrix: X = scale * working matrix
     uint32_t *active;          // per matrix: 0 = skipped by the products and by what follows
@@ -119,9 +125,10 @@ struct NsBatchArgs {
     int32_t tile0, n_tiles;
 };
 constexpr int kNsTileI = 64, kNsTileJ = 128;  // an element-wise tile of the working matrix
-int launch_ns_norm(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
-int launch_ns_gather(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
-int launch_ns_finish(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, cudaStream_t stream);
+// turned: some array of the list is contiguous along the short side
+int launch_ns_norm(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, bool turned, cudaStream_t stream);
+int launch_ns_gather(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, bool turned, cudaStream_t stream);
+int launch_ns_finish(const NsElementwise &w, const NsBatchArgs &b, const int32_t *d_tile_matrix, bool step, bool turned, cudaStream_t stream);
 
 // ---- matrices with a short side of at most 64 (ns_small.cu) ----------------------------------
 constexpr int kNsSmallSide = 64;

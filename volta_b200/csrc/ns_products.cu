@@ -53,7 +53,7 @@ namespace vb {
 namespace {
 
 constexpr int BM = 128;
-constexpr int BK = 64;  // f16 elements: one 128-byte swizzle row
+constexpr int BK = kNsKBlock;  // f16 elements: one 128-byte swizzle row
 constexpr int UMMA_K = 16;
 constexpr int kBoxBytes = 64 * BK * 2;
 constexpr int kRows128Bytes = 128 * BK * 2;
@@ -113,7 +113,7 @@ __device__ __forceinline__ uint32_t make_idesc(bool b_mn_major, int m, int n)
 
 struct Tile {
     const NsProduct *p;
-    int m0, n0, k_blocks, matrix;
+    int m0, n0, kb0, kb1, matrix, part, parts;
     uint32_t after;
     bool mirror, b_mn, skipped;
 };
@@ -121,7 +121,8 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
 {
     Tile ti;
     ti.p = l.problems;
-    ti.m0 = ti.n0 = ti.k_blocks = ti.matrix = 0;
+    ti.m0 = ti.n0 = ti.kb0 = ti.kb1 = ti.matrix = ti.parts = 0;
+    ti.part = -1;
     ti.after = 0;
     ti.mirror = ti.b_mn = false;
     ti.skipped = true;
@@ -134,7 +135,10 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
         ti.mirror = tile.mirror != 0;
         ti.after = tile.after;
         ti.matrix = p->matrix;
-        ti.k_blocks = p->K / BK;
+        ti.kb0 = tile.kb0;
+        ti.kb1 = tile.kb1;
+        ti.part = tile.part;
+        ti.parts = tile.parts;
         ti.b_mn = (p->flags & NS_B_MN_MAJOR) != 0;
         ti.skipped = __ldcg(active + p->matrix) == 0u;
     }
@@ -147,7 +151,10 @@ __device__ __forceinline__ Tile uniform_tile(const Tile &t)
     u.p = uniform(const_cast<NsProduct *>(t.p));
     u.m0 = uniform(t.m0);
     u.n0 = uniform(t.n0);
-    u.k_blocks = uniform(t.k_blocks);
+    u.kb0 = uniform(t.kb0);
+    u.kb1 = uniform(t.kb1);
+    u.part = uniform(t.part);
+    u.parts = uniform(t.parts);
     u.matrix = uniform(t.matrix);
     u.after = uniform(t.after);
     const int flags = uniform((t.mirror ? 1 : 0) | (t.b_mn ? 2 : 0) | (t.skipped ? 4 : 0));
@@ -409,7 +416,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             }
             asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what other SMs stored
 #pragma unroll 1
-            for (int kb = 0; kb < ti.k_blocks; ++kb) {
+            for (int kb = ti.kb0; kb < ti.kb1; ++kb) {
                 if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, wait_limit))) {
                     ok = false;
                     break;
@@ -456,14 +463,16 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 // B's descriptor differs by its major-ness in the fields above the address and in the step of a k slice
                 const uint64_t desc_b0 = ti.b_mn ? desc_mn : desc_k;
                 const uint32_t step_b = ti.b_mn ? 2048 >> 4 : 32 >> 4;
-                for (int k0 = 0; k0 < ti.k_blocks && ok; k0 += C::kChunkBlocks) {
-                    const int k1 = min(k0 + C::kChunkBlocks, ti.k_blocks);
+                // (a tile that sums pieces has nothing to multiply: one round that hands the accumulator over)
+                for (int k0 = ti.kb0; (k0 < ti.kb1 || k0 == ti.kb0) && ok; k0 += C::kChunkBlocks) {
+                    const int k1 = min(k0 + C::kChunkBlocks, ti.kb1);
                     if (!__all_sync(0xffffffffu, mbar_wait(&bars->tmem_empty[acc], acc_phase ^ 1u, abort_flag, wait_limit))) {
                         ok = false;
                         break;
                     }
                     tcgen05_fence_after();
                     const uint32_t tmem_d = tmem + (uint32_t)(acc * C::BN);
+                    if (k0 >= k1 && elected) tcgen05_commit<kCtas>(&bars->tmem_full[acc]);
                     bool ready = false;
 #pragma unroll 1
                     for (int kb = k0; kb < k1; ++kb) {
@@ -537,7 +546,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 if (p->n_terms > 0) prefetch_map(&p->map_term[0]);
                 prefetch_map(&p->map_d);
             }
-            if (inside && drain.per_piece > 0) {  // the first term: its matrix must be stored
+            if (inside && !(ti.part >= 0 && ti.parts == 0) && drain.per_piece > 0) {  // the first term: its matrix must be stored
                 if (!__all_sync(0xffffffffu, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device,
                                                          abort_flag, wait_limit))) {
                     ok = false;
@@ -561,11 +570,14 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 tcgen05_fence_after();
                 return full;
             };
-            if (kPlanes == 2) {
-                float sum[kCols];
+            const bool piece = ti.part >= 0 && ti.parts == 0;
+            float *const slot = launch.partials + (ti.part >= 0 ? (int64_t)ti.part * BM * BM : 0) +
+                                (int64_t)(quarter * 32 + lane) * BM + col_half * kCols;
+            float sum[kPlanes == 2 ? kCols : 1];
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
-                const int chunks = (ti.k_blocks + C::kChunkBlocks - 1) / C::kChunkBlocks;
+            for (int j = 0; j < (kPlanes == 2 ? kCols : 1); ++j) sum[j] = 0.0f;
+            if (kPlanes == 2) {
+                const int chunks = (ti.kb1 - ti.kb0 + C::kChunkBlocks - 1) / C::kChunkBlocks;
                 for (int c = 0; c + 1 < chunks && ok; ++c) {
                     ok = wait_acc();
                     if (!ok) break;
@@ -574,34 +586,74 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                         uint32_t v[32];
                         tmem_ld_32x32_sync(my_tmem + (uint32_t)(acc * C::BN + cc * 32), v);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[cc * 32 + j] += __uint_as_float(v[j]);
+                        for (int j = 0; j < 32; ++j) sum[kPlanes == 2 ? cc * 32 + j : 0] += __uint_as_float(v[j]);
                     }
                     drained(acc);
                     acc ^= 1;
                     acc_phase ^= acc == 0 ? 1u : 0u;
                 }
-                if (ok) ok = wait_acc();
-                if (!ok) break;
-                // the last piece joins, and the sum goes back into this warp's part of the accumulator, to be
-                // drained from there: the sum and the drain do not fit the registers together
+            }
+            if (ok) ok = wait_acc();
+            if (!ok) break;
+            const uint32_t acc_tmem = my_tmem + (uint32_t)(acc * C::BN);
+            if (kCtas == 1 && ti.parts > 0) {
+                // the pieces in order, into this warp's part of the (unused) accumulator
+                if (!__all_sync(0xffffffffu, wait_stored(launch.stored + ti.matrix, ti.after * kArrivals, error.device,
+                                                         abort_flag, wait_limit))) {
+                    ok = false;
+                    break;
+                }
+#pragma unroll 1
+                for (int cc = 0; cc < kCols / 32; ++cc) {
+                    float t[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) t[j] = 0.0f;
+#pragma unroll 2
+                    for (int k = 0; k < ti.parts; ++k) {
+                        const float4 *from = reinterpret_cast<const float4 *>(slot + (int64_t)k * BM * BM + cc * 32);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const float4 x = __ldcg(from + q);  // written by other SMs in this launch
+                            t[4 * q] += x.x, t[4 * q + 1] += x.y, t[4 * q + 2] += x.z, t[4 * q + 3] += x.w;
+                        }
+                    }
+                    uint32_t v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(t[j]);
+                    tmem_st_32x32(acc_tmem + (uint32_t)(cc * 32), v);
+                }
+                tmem_st_wait();
+            } else if (kPlanes == 2 || (kCtas == 1 && piece)) {
+                // two planes: the last part joins, and the sum goes back into this warp's part of the accumulator, to be
+                // drained from there: the sum and the drain do not fit the registers together.  A piece of a cut
+                // contraction goes to its slot instead.
 #pragma unroll
                 for (int cc = 0; cc < kCols / 32; ++cc) {
                     uint32_t v[32];
-                    tmem_ld_32x32_sync(my_tmem + (uint32_t)(acc * C::BN + cc * 32), v);
+                    tmem_ld_32x32_sync(acc_tmem + (uint32_t)(cc * 32), v);
+                    if (kPlanes == 2) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[cc * 32 + j] + __uint_as_float(v[j]));
-                    tmem_st_32x32(my_tmem + (uint32_t)(acc * C::BN + cc * 32), v);
+                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[kPlanes == 2 ? cc * 32 + j : 0] + __uint_as_float(v[j]));
+                    }
+                    if (kCtas == 1 && piece) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t o[8] = {v[8 * q], v[8 * q + 1], v[8 * q + 2], v[8 * q + 3],
+                                                   v[8 * q + 4], v[8 * q + 5], v[8 * q + 6], v[8 * q + 7]};
+                            st_global_256(slot + cc * 32 + q * 8, o);
+                        }
+                    } else {
+                        tmem_st_32x32(acc_tmem + (uint32_t)(cc * 32), v);
+                    }
                 }
                 tmem_st_wait();
-            } else {
-                ok = wait_acc();
-                if (!ok) break;
             }
-            if (inside) ok = drain.run(my_tmem + (uint32_t)(acc * C::BN), mult, abort_flag, wait_limit, [&] { drained(acc); });
+            if (inside && !piece) ok = drain.run(acc_tmem, mult, abort_flag, wait_limit, [&] { drained(acc); });
             else drained(acc);
             acc ^= 1;
             acc_phase ^= acc == 0 ? 1u : 0u;
-            if (ok) {  // this warp's part of D is in memory, for TMA loads of other SMs
+            if (ok) {  // this warp's part of D (or of a slot) is in memory, for other SMs
+                __syncwarp();
                 if (lane == 0) {
                     bulk_wait_all();
                     asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(launch.stored + ti.matrix) : "memory");

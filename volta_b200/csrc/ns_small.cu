@@ -55,7 +55,6 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b)
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-__device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 
 // f += c * (16 values of one row of a block, columns col .. col + 15, all planes)
 template <int kPlanes>
@@ -202,53 +201,12 @@ struct Share {
         count = left < 0 ? 0 : left < 8 ? left : 8;
     }
     __device__ __forceinline__ int64_t offset(const NsArray &a, int i, int j) const { return (int64_t)i * a.si + (int64_t)(j0 + j) * a.sj; }
+    __device__ __forceinline__ int64_t step(const NsArray &a) const { return along_i ? a.si : a.sj; }
     // a vector access runs along the array's own direction
     __device__ __forceinline__ bool vec(const NsArray &a, bool aligned) const { return aligned && walks_i(a) == along_i; }
     __device__ __forceinline__ void write(int type, const NsArray &a, bool aligned, int i, int j, int count, const float (&v)[8]) const
     {
         store8(type, a.ptr, offset(a, i, j), along_i ? a.si : a.sj, count, vec(a, aligned), v);
-    }
-};
-
-// 8 elements as they lie in memory (whole and aligned octets) or as f32: loads first, conversions later, so that
-// a thread has several octets on their way.
-struct Raw {
-    uint4 q[2];
-    bool packed;
-    __device__ __forceinline__ void load(int type, const NsArray &a, const Share &s, bool aligned, int i, int j, int count)
-    {
-        packed = count == 8 && s.vec(a, aligned);
-        if (packed) {
-            const char *p = static_cast<const char *>(a.ptr) + s.offset(a, i, j) * (type == VB_DTYPE_F32 ? 4 : 2);
-            q[0] = *reinterpret_cast<const uint4 *>(p);
-            if (type == VB_DTYPE_F32) q[1] = reinterpret_cast<const uint4 *>(p)[1];
-        }
-    }
-    __device__ __forceinline__ void get(int type, const NsArray &a, const Share &s, int i, int j, int count, float (&v)[8]) const
-    {
-        if (!packed) {
-            load8(type, a.ptr, s.offset(a, i, j), s.along_i ? a.si : a.sj, count, false, v);
-            return;
-        }
-        if (type == VB_DTYPE_F32) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                v[4 * k] = __uint_as_float(q[k].x), v[4 * k + 1] = __uint_as_float(q[k].y);
-                v[4 * k + 2] = __uint_as_float(q[k].z), v[4 * k + 3] = __uint_as_float(q[k].w);
-            }
-        } else {
-            const uint32_t h[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (type == VB_DTYPE_BF16) {
-                    v[2 * k] = __uint_as_float(h[k] << 16);
-                    v[2 * k + 1] = __uint_as_float(h[k] & 0xffff0000u);
-                } else {
-                    const float2 x = unpack_half(h[k]);
-                    v[2 * k] = x.x, v[2 * k + 1] = x.y;
-                }
-            }
-        }
     }
 };
 
@@ -265,8 +223,8 @@ __device__ __forceinline__ void for_u(const NsElementwise &w, const NsMatrixArg 
             if (o >= s.octets()) break;
             int i, j, count;
             s.locate(o, i, j, count);
-            g[k].load(w.types[0], a.a[0], s, a.direct & 1u, i, j, count);
-            if (kStep) v[kStep ? k : 0].load(w.types[1], a.a[1], s, a.direct & 2u, i, j, count);
+            g[k].load(w.types[0], a.a[0].ptr, s.offset(a.a[0], i, j), count, s.vec(a.a[0], a.direct & 1u));
+            if (kStep) v[kStep ? k : 0].load(w.types[1], a.a[1].ptr, s.offset(a.a[1], i, j), count, s.vec(a.a[1], a.direct & 2u));
         }
 #pragma unroll
         for (int k = 0; k < kInFlight; ++k) {
@@ -275,9 +233,9 @@ __device__ __forceinline__ void for_u(const NsElementwise &w, const NsMatrixArg 
             int i, j, count;
             s.locate(o, i, j, count);
             float gg[8], vv[8], u[8];
-            g[k].get(w.types[0], a.a[0], s, i, j, count, gg);
+            g[k].get(w.types[0], a.a[0].ptr, s.offset(a.a[0], i, j), s.step(a.a[0]), count, gg);
             if (kStep) {
-                v[kStep ? k : 0].get(w.types[1], a.a[1], s, i, j, count, vv);
+                v[kStep ? k : 0].get(w.types[1], a.a[1].ptr, s.offset(a.a[1], i, j), s.step(a.a[1]), count, vv);
                 momentum8(w, gg, vv, u);
             } else {
 #pragma unroll
@@ -579,7 +537,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 int i, j, count;
                 if (o0 + k * kThreads >= out.octets()) break;
                 out.locate(o0 + k * kThreads, i, j, count);
-                p[k].load(w.types[kOut], dst, out, (a.direct >> kOut) & 1u, i, j, count);
+                p[k].load(w.types[kOut], dst.ptr, out.offset(dst, i, j), count, out.vec(dst, (a.direct >> kOut) & 1u));
             }
 #pragma unroll
             for (int k = 0; k < kInFlight; ++k) {
@@ -612,7 +570,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 }
                 if (kStep) {
                     float pp[8];
-                    p[kStep ? k : 0].get(w.types[kOut], dst, out, i, j, count, pp);
+                    p[kStep ? k : 0].get(w.types[kOut], dst.ptr, out.offset(dst, i, j), out.step(dst), count, pp);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] = fmaf(-rate, f[e] * d.final_scale, pp[e] * w.decay);
                 } else {
