@@ -341,14 +341,14 @@ struct Carver {
 
 // Calls fn(m0, n0, mirror) for every tile of a product that is computed; returns their number.
 template <typename Fn>
-uint32_t for_tiles(const NsProduct &pr, int shape, Fn &&fn)
+uint32_t for_tiles(const NsProduct &pr, int shape, int planes, Fn &&fn)
 {
     int bm, bn;
-    ns_tile_extent(shape, &bm, &bn);
+    ns_tile_extent(shape, planes, &bm, &bn);
     const bool symmetric = (pr.flags & NS_B_MN_MAJOR) == 0;
     uint32_t count = 0;
     for (int m0 = 0; m0 < pr.M; m0 += bm)
-        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn, ++count) fn(m0, n0, symmetric && n0 > m0);
+        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn, ++count) fn(m0, n0, symmetric && n0 >= m0 + bm);
     return count;
 }
 
@@ -362,30 +362,33 @@ int gram_parts(const NsProduct &pr, int shape, uint32_t stage_tiles, int sm_coun
     return std::max(1, std::min(pr.K / kNsKBlock / 8, sm_count / (int)stage_tiles));
 }
 
-// The shape whose stages take less time if every stage is waited for: whole rounds of tiles over the
-// device's CTAs (pairs), a round costing its FLOPs per SM.  A 128 x 128 tile reads twice the
-// operands per FLOP and, with all SMs busy, runs at 0.6 of the pair's rate.
-int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t> &stage_begin, int sm_count)
+// The shape whose stages take less time if every stage is waited for: whole rounds of tiles over the device's
+// CTAs (pairs), at the measured cycles of a tile per element of the contraction, plus what a stage costs
+// besides (signals, first loads, epilogue: about 12000 cycles).  One plane: a 128 x 128 tile takes 10.5 cycles
+// (issue bound), a pair's 256 x 256 one 11.9 (bound by L2); two planes 18.7 and, 256 x 128, 18.4.
+int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t> &stage_begin, int planes, int sm_count)
 {
+    const double cycles[2][2] = {{11.9, 10.5}, {18.4, 18.7}}, per_stage = 12000.0;
     double cost[2] = {0.0, 0.0};
     for (int shape = 0; shape < 2; ++shape) {
-        const double groups = shape == NS_TILE_PAIR_256 ? sm_count / 2 : sm_count;
-        const double tile = shape == NS_TILE_PAIR_256 ? 2.0 : 1.0 / 0.6;  // time of a tile per k
+        const double groups = shape == NS_TILE_PAIR ? sm_count / 2 : sm_count;
         for (size_t k = 0; k + 1 < stage_begin.size(); ++k) {
             double work = 0.0, longest = 0.0;
             uint32_t tiles = 0;
+            bool cut = false;
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) tiles += for_tiles(problems[q], shape, planes, [](int, int, bool) {});
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
-                const uint32_t count = for_tiles(problems[q], shape, [](int, int, bool) {});
-                tiles += count;
-                work += (double)count * problems[q].K;
-                longest = std::max(longest, (double)problems[q].K);
+                const int parts = gram_parts(problems[q], shape, tiles, sm_count);
+                cut = cut || parts > 1;
+                work += (double)for_tiles(problems[q], shape, planes, [](int, int, bool) {}) * problems[q].K;
+                longest = std::max(longest, (double)problems[q].K / parts);
             }
             if (tiles == 0) continue;
             const double rounds = std::ceil(tiles / groups), mean = work / tiles;
-            cost[shape] += tile * std::max(longest, rounds * mean);
+            cost[shape] += per_stage * (cut ? 2 : 1) + cycles[planes - 1][shape] * std::max(longest, cut ? work / groups : rounds * mean);
         }
     }
-    return cost[NS_TILE_PAIR_256] <= cost[NS_TILE_128] ? NS_TILE_PAIR_256 : NS_TILE_128;
+    return cost[NS_TILE_PAIR] <= cost[NS_TILE_128] ? NS_TILE_PAIR : NS_TILE_128;
 }
 
 int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
@@ -529,7 +532,9 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                     if (round == 1) {
                         const int64_t outer = (int64_t)p->planes * d.np;
                         VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, outer, NS_MAP_ROWS));
-                        VB_TRY(make_ns_map(&q.map_b, address(pr.B), pr.update ? q.N : q.K, outer, pr.update ? NS_MAP_MN : NS_MAP_ROWS));
+                        const bool narrow = p->planes == 2 && p->shape == NS_TILE_PAIR;  // 64 rows of B per CTA
+                        VB_TRY(make_ns_map(&q.map_b, address(pr.B), pr.update ? q.N : q.K, outer,
+                                           pr.update ? (narrow ? NS_MAP_MN_64 : NS_MAP_MN) : (narrow ? NS_MAP_ROWS_64 : NS_MAP_ROWS)));
                         if (pr.E >= 0) VB_TRY(make_ns_map(&q.map_term[0], address(pr.E), q.N, outer, NS_MAP_PIECE));
                         if (pr.F >= 0) VB_TRY(make_ns_map(&q.map_term[1], address(pr.F), q.N, outer, NS_MAP_PIECE));
                         VB_TRY(make_ns_map(&q.map_d, address(pr.D), q.N, outer, NS_MAP_PIECE));
@@ -543,11 +548,11 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                              [](const NsProduct &a, const NsProduct &b) { return a.K > b.K; });
         }
         stage_begin.push_back(problems.size());
-        p->shape = pick_shape(problems, stage_begin, p->eng->sm_count);
+        p->shape = pick_shape(problems, stage_begin, p->planes, p->eng->sm_count);
         tile_list.clear();
         std::vector<uint32_t> done((size_t)n, 0), stage_done((size_t)n, 0);
         size_t widest = 0;
-        auto count_tiles = [&](const NsProduct &pr) { return for_tiles(pr, p->shape, [](int, int, bool) {}); };
+        auto count_tiles = [&](const NsProduct &pr) { return for_tiles(pr, p->shape, p->planes, [](int, int, bool) {}); };
         std::vector<uint32_t> stage_tiles(n_stages, 0);
         for (size_t k = 0; k < n_stages; ++k)
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) stage_tiles[k] += count_tiles(problems[q]);
@@ -575,7 +580,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                 const int parts = gram_parts(pr, p->shape, stage_tiles[k], p->eng->sm_count);
                 int32_t slot = slot0[i];
                 uint32_t count = 0;
-                for_tiles(pr, p->shape, [&](int m0, int n0, bool mirror) {
+                for_tiles(pr, p->shape, p->planes, [&](int m0, int n0, bool mirror) {
                     if (parts == 1) {
                         tile_list.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, done[i], 0, blocks, -1, 0});
                         ++count;
@@ -605,7 +610,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             VB_CUDA(cudaMemcpyAsync(d_problems, problems.data(), problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
             int bm, bn;
-            ns_tile_extent(p->shape, &bm, &bn);
+            ns_tile_extent(p->shape, p->planes, &bm, &bn);
             double stage_flops = 0.0;  // of the largest product
             for (size_t q = 0; q < problems.size(); ++q)
                 stage_flops = std::max(stage_flops, 2.0 * (double)problems[q].M * problems[q].N * problems[q].K * 3.0);

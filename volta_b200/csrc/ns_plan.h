@@ -27,7 +27,7 @@ enum NsProductFlags {
 struct alignas(128) NsProduct {
     // tensor maps, see make_ns_map
     CUtensorMap map_a;         // operand, NS_MAP_ROWS
-    CUtensorMap map_b;         // operand, NS_MAP_ROWS or NS_MAP_MN
+    CUtensorMap map_b;         // operand, NS_MAP_ROWS or NS_MAP_MN (or their 64-wide forms)
     CUtensorMap map_term[2];   // E and F, NS_MAP_PIECE
     CUtensorMap map_d;         // D, NS_MAP_PIECE
     CUtensorMap map_mirror;    // D, NS_MAP_MIRROR
@@ -62,10 +62,10 @@ struct NsLaunch {
 
 // Tile shapes of the product kernel.
 enum NsTileShape {
-    NS_TILE_PAIR_256 = 0,  // two CTAs, 256 x 256
-    NS_TILE_128 = 1        // one CTA, 128 x 128
+    NS_TILE_PAIR = 0,  // two CTAs, 256 x 256 (two planes: 256 x 128)
+    NS_TILE_128 = 1    // one CTA, 128 x 128
 };
-void ns_tile_extent(int shape, int *bm, int *bn);
+void ns_tile_extent(int shape, int planes, int *bm, int *bn);
 // Where a kernel reports a wait that ran out: a device word later kernels look at, a mapped one for the host.
 struct NsError {
     uint32_t *device, *host;
@@ -78,7 +78,8 @@ enum NsMap {
     NS_MAP_ROWS = 0,   // 64 x 128 boxes, 128-byte swizzle: 128 rows x 64 k of an operand
     NS_MAP_MN = 1,     // 64 x 64 x 2 boxes of the view [inner / 64][outer][64], same swizzle: 64 k x 128 columns
     NS_MAP_PIECE = 2,  // 64 x 32 boxes, same swizzle: what an epilogue warp reads or writes at once
-    NS_MAP_MIRROR = 3  // 32 x 64 boxes: the same piece transposed
+    NS_MAP_MIRROR = 3, // 32 x 64 boxes: the same piece transposed
+    NS_MAP_ROWS_64 = 4, NS_MAP_MN_64 = 5  // as the first two, 64 rows or columns
 };
 int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int kind);
 

@@ -24,7 +24,10 @@
 //
 // Warp roles as in ns_gemm_tc.cu: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue with two
 // accumulators.  Two shapes:
-//   256 x 256 by a CTA pair (cta_group::2): half the operand traffic per FLOP
+//   256 x 256 (two planes: 256 x 128) by a CTA pair (cta_group::2): half the operand traffic per FLOP.  With one plane
+//             that traffic (L2 to shared memory) is what bounds large products: with B not loaded at all they ran
+//             at 1350 instead of 1072 TFLOP/s.  Two planes do three products on what they load; there 256 columns
+//             only cost registers (the sums spilled) and parallelism (2048 x 2048 f32: 870 us against 785)
 //   128 x 128 by one CTA: four times as many tiles, for lists that would leave SMs idle
 // (the planner picks, see pick_shape).
 //
@@ -67,9 +70,10 @@ constexpr int kMaxStages = 4;
 
 template <int kCtas, int kPlanes>
 struct Cfg {
-    static constexpr int BN = 128 * kCtas;
+    static constexpr int BN = kCtas == 2 && kPlanes == 1 ? 256 : 128;  // columns of a tile
+    static constexpr int kBRows = BN / kCtas;                           // rows of B a CTA stages
     static constexpr int kStages = kPlanes == 1 ? 4 : 2;
-    static constexpr int kPlaneBytes = 2 * kRows128Bytes;  // 128 rows of A, 128 rows of B
+    static constexpr int kPlaneBytes = kRows128Bytes + kBRows * BK * 2;  // 128 rows of A, kBRows of B
     static constexpr int kStageBytes = kPlanes * kPlaneBytes;
     static constexpr int kTmemCols = 2 * BN;
     static constexpr int kChunkBlocks = kPlanes == 1 ? 1 << 20 : 128 / BK;  // k blocks one accumulator takes
@@ -402,7 +406,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             const Tile ti = uniform_tile(next);
             next = fetch_tile(launch, active, t + n_groups);
             if (ti.skipped) continue;
-            const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * 128;
+            const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * C::kBRows;
             const int plane_rows = uniform(ti.p->plane_rows);
             const CUtensorMap *map_a = &ti.p->map_a, *map_b = &ti.p->map_b;
             if (elected) {
@@ -743,7 +747,11 @@ int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, i
 
 }  // namespace
 
-void ns_tile_extent(int shape, int *bm, int *bn) { *bm = *bn = shape == NS_TILE_PAIR_256 ? 256 : 128; }
+void ns_tile_extent(int shape, int planes, int *bm, int *bn)
+{
+    *bm = shape == NS_TILE_PAIR ? 256 : 128;
+    *bn = shape == NS_TILE_PAIR && planes == 1 ? 256 : 128;
+}
 
 int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int kind)
 {
@@ -756,11 +764,12 @@ int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer
             fn = reinterpret_cast<EncodeTiledFn>(sym);
     }
     if (!fn) return fail(VB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    const bool view = kind == NS_MAP_MN;
+    const bool view = kind == NS_MAP_MN || kind == NS_MAP_MN_64;
     cuuint32_t estr[3] = {1, 1, 1};
     cuuint64_t dims[3] = {view ? 64 : (cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)(inner / 64)};
     cuuint64_t strides[2] = {(cuuint64_t)inner * 2, 128};
-    cuuint32_t box[3] = {kind == NS_MAP_MIRROR ? 32u : 64u, kind == NS_MAP_ROWS ? 128u : kind == NS_MAP_PIECE ? 32u : 64u, 2};
+    cuuint32_t box[3] = {kind == NS_MAP_MIRROR ? 32u : 64u, kind == NS_MAP_ROWS ? 128u : kind == NS_MAP_PIECE ? 32u : 64u,
+                         kind == NS_MAP_MN_64 ? 1u : 2u};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, view ? 3 : 2, const_cast<void *>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, kind == NS_MAP_MIRROR ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -772,7 +781,7 @@ int launch_ns_products(const NsLaunch &l, int shape, int planes, const uint32_t 
                        int sm_count, cudaStream_t stream, uint32_t wait_limit, bool withhold)
 {
     if (l.n_tiles <= 0) return VB_OK;
-    if (shape == NS_TILE_PAIR_256)
+    if (shape == NS_TILE_PAIR)
         return planes == 2 ? launch_variant<2, 2>(l, d_active, error, sm_count, stream, wait_limit, withhold)
                            : launch_variant<2, 1>(l, d_active, error, sm_count, stream, wait_limit, withhold);
     return planes == 2 ? launch_variant<1, 2>(l, d_active, error, sm_count, stream, wait_limit, withhold)
