@@ -339,7 +339,7 @@ struct Carver {
     }
 };
 
-// Calls fn(m0, n0, mirror) for every tile of a product that is computed; returns their number.
+// Calls fn(m0, n0, flags) for every tile of a product that is computed; returns their number.
 template <typename Fn>
 uint32_t for_tiles(const NsProduct &pr, int shape, int planes, Fn &&fn)
 {
@@ -348,7 +348,8 @@ uint32_t for_tiles(const NsProduct &pr, int shape, int planes, Fn &&fn)
     const bool symmetric = (pr.flags & NS_B_MN_MAJOR) == 0;
     uint32_t count = 0;
     for (int m0 = 0; m0 < pr.M; m0 += bm)
-        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn, ++count) fn(m0, n0, symmetric && n0 >= m0 + bm);
+        for (int n0 = symmetric ? m0 : 0; n0 < pr.N; n0 += bn, ++count)
+            fn(m0, n0, (symmetric && n0 >= m0 + bm ? NS_TILE_MIRROR : 0) | ((pr.flags & NS_SAME) && n0 == m0 && bm == bn ? NS_TILE_SHARED : 0));
     return count;
 }
 
@@ -376,11 +377,11 @@ int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t>
             double work = 0.0, longest = 0.0;
             uint32_t tiles = 0;
             bool cut = false;
-            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) tiles += for_tiles(problems[q], shape, planes, [](int, int, bool) {});
+            for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) tiles += for_tiles(problems[q], shape, planes, [](int, int, int) {});
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) {
                 const int parts = gram_parts(problems[q], shape, tiles, sm_count);
                 cut = cut || parts > 1;
-                work += (double)for_tiles(problems[q], shape, planes, [](int, int, bool) {}) * problems[q].K;
+                work += (double)for_tiles(problems[q], shape, planes, [](int, int, int) {}) * problems[q].K;
                 longest = std::max(longest, (double)problems[q].K / parts);
             }
             if (tiles == 0) continue;
@@ -528,7 +529,8 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                     q.scale_power = pr.scale_power;
                     q.scale = p->ew.scale + i;
                     q.matrix = (int32_t)i;
-                    q.flags = (pr.update ? NS_B_MN_MAJOR : 0) | (pr.gram ? NS_GRAM : 0);
+                    q.flags = (pr.update ? NS_B_MN_MAJOR : 0) | (pr.gram ? NS_GRAM : 0) |
+                              (pr.A == pr.B && !pr.update ? NS_SAME : 0);
                     if (round == 1) {
                         const int64_t outer = (int64_t)p->planes * d.np;
                         VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, outer, NS_MAP_ROWS));
@@ -552,7 +554,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         tile_list.clear();
         std::vector<uint32_t> done((size_t)n, 0), stage_done((size_t)n, 0);
         size_t widest = 0;
-        auto count_tiles = [&](const NsProduct &pr) { return for_tiles(pr, p->shape, p->planes, [](int, int, bool) {}); };
+        auto count_tiles = [&](const NsProduct &pr) { return for_tiles(pr, p->shape, p->planes, [](int, int, int) {}); };
         std::vector<uint32_t> stage_tiles(n_stages, 0);
         for (size_t k = 0; k < n_stages; ++k)
             for (size_t q = stage_begin[k]; q < stage_begin[k + 1]; ++q) stage_tiles[k] += count_tiles(problems[q]);
@@ -580,15 +582,15 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                 const int parts = gram_parts(pr, p->shape, stage_tiles[k], p->eng->sm_count);
                 int32_t slot = slot0[i];
                 uint32_t count = 0;
-                for_tiles(pr, p->shape, p->planes, [&](int m0, int n0, bool mirror) {
+                for_tiles(pr, p->shape, p->planes, [&](int m0, int n0, int flags) {
                     if (parts == 1) {
-                        tile_list.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, done[i], 0, blocks, -1, 0});
+                        tile_list.push_back({(int32_t)q, m0, n0, flags, done[i], 0, blocks, -1, 0});
                         ++count;
                         return;
                     }
-                    sums.push_back({(int32_t)q, m0, n0, mirror ? 1 : 0, 0, 0, 0, slot, parts});
+                    sums.push_back({(int32_t)q, m0, n0, flags, 0, 0, 0, slot, parts});
                     for (int part = 0; part < parts; ++part, ++count)
-                        tile_list.push_back({(int32_t)q, m0, n0, 0, done[i], blocks * part / parts, blocks * (part + 1) / parts, slot++, 0});
+                        tile_list.push_back({(int32_t)q, m0, n0, flags & NS_TILE_SHARED, done[i], blocks * part / parts, blocks * (part + 1) / parts, slot++, 0});
                 });
                 stage_done[i] += count;
             }

@@ -22,7 +22,8 @@ constexpr int kNsPad = 128;  // sides of the working matrices are multiples of t
 // E and F (f16, leading dimension and planes of D; may be null) are read at D's position.
 enum NsProductFlags {
     NS_B_MN_MAJOR = 1,  // B is stored [k][n] (the working matrix X); otherwise [n][k]
-    NS_GRAM = 2         // X X^T: the contraction runs over the long side
+    NS_GRAM = 2,        // X X^T: the contraction runs over the long side
+    NS_SAME = 4         // A and B are one matrix
 };
 struct alignas(128) NsProduct {
     // tensor maps, see make_ns_map
@@ -40,9 +41,13 @@ struct alignas(128) NsProduct {
     int32_t matrix;          // index into the activity words
     int32_t flags;
 };
+enum NsTileFlags {
+    NS_TILE_MIRROR = 1,  // symmetric product: the tile is also stored transposed
+    NS_TILE_SHARED = 2   // A times its own transpose, on the diagonal: the rows of B are those of A, staged once
+};
 struct NsTile {
     int32_t problem, m0, n0;
-    int32_t mirror;   // symmetric product: the tile is also stored transposed
+    int32_t flags;    // NsTileFlags
     uint32_t after;   // tiles of the matrix's earlier stages: all of them must be stored before this one starts
     int32_t kb0, kb1; // blocks of 64 of the contraction
     // A contraction cut into pieces (128 x 128 tiles): a piece (part >= 0, parts == 0) stores its f32 accumulator in

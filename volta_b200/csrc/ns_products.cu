@@ -119,7 +119,7 @@ struct Tile {
     const NsProduct *p;
     int m0, n0, kb0, kb1, matrix, part, parts;
     uint32_t after;
-    bool mirror, b_mn, skipped;
+    bool mirror, shared, b_mn, skipped;
 };
 __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *active, int t)
 {
@@ -128,7 +128,7 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
     ti.m0 = ti.n0 = ti.kb0 = ti.kb1 = ti.matrix = ti.parts = 0;
     ti.part = -1;
     ti.after = 0;
-    ti.mirror = ti.b_mn = false;
+    ti.mirror = ti.shared = ti.b_mn = false;
     ti.skipped = true;
     if (t < l.n_tiles) {
         const NsTile tile = l.tiles[t];
@@ -136,7 +136,8 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
         ti.p = p;
         ti.m0 = tile.m0;
         ti.n0 = tile.n0;
-        ti.mirror = tile.mirror != 0;
+        ti.mirror = (tile.flags & NS_TILE_MIRROR) != 0;
+        ti.shared = (tile.flags & NS_TILE_SHARED) != 0;
         ti.after = tile.after;
         ti.matrix = p->matrix;
         ti.kb0 = tile.kb0;
@@ -161,8 +162,8 @@ __device__ __forceinline__ Tile uniform_tile(const Tile &t)
     u.parts = uniform(t.parts);
     u.matrix = uniform(t.matrix);
     u.after = uniform(t.after);
-    const int flags = uniform((t.mirror ? 1 : 0) | (t.b_mn ? 2 : 0) | (t.skipped ? 4 : 0));
-    u.mirror = flags & 1, u.b_mn = flags & 2, u.skipped = flags & 4;
+    const int flags = uniform((t.mirror ? 1 : 0) | (t.b_mn ? 2 : 0) | (t.skipped ? 4 : 0) | (t.shared ? 8 : 0));
+    u.mirror = flags & 1, u.b_mn = flags & 2, u.skipped = flags & 4, u.shared = flags & 8;
     return u;
 }
 
@@ -427,12 +428,14 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 }
                 if (elected && !withhold) {  // withheld: nothing is announced or staged, the bounded waits run out
                     const uint32_t slot = slots + (uint32_t)stage * C::kStageBytes, full = full0 + 8 * stage;
-                    if (cta_rank == 0) mbar_expect_tx(my_full0 + 8 * stage, kCtas * C::kStageBytes);
+                    if (cta_rank == 0)
+                        mbar_expect_tx(my_full0 + 8 * stage, kCtas * (ti.shared ? kPlanes * kRows128Bytes : C::kStageBytes));
 #pragma unroll
                     for (int pl = 0; pl < kPlanes; ++pl) {
                         load_rows<kCtas>(slot + pl * C::kPlaneBytes, map_a, false, a_row0, kb * BK, pl * plane_rows, full);
-                        load_rows<kCtas>(slot + pl * C::kPlaneBytes + kRows128Bytes, map_b, ti.b_mn, b_row0, kb * BK,
-                                         pl * plane_rows, full);
+                        if (!ti.shared)
+                            load_rows<kCtas>(slot + pl * C::kPlaneBytes + kRows128Bytes, map_b, ti.b_mn, b_row0, kb * BK,
+                                             pl * plane_rows, full);
                     }
                 }
                 if (++stage == C::kStages) {
@@ -465,7 +468,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 if (ti.skipped) continue;
                 const uint32_t idesc = make_idesc(ti.b_mn, BM * kCtas, C::BN);
                 // B's descriptor differs by its major-ness in the fields above the address and in the step of a k slice
-                const uint64_t desc_b0 = ti.b_mn ? desc_mn : desc_k;
+                const uint64_t desc_b0 = (ti.b_mn ? desc_mn : desc_k) + (ti.shared ? 0 : kRows128Bytes >> 4);
                 const uint32_t step_b = ti.b_mn ? 2048 >> 4 : 32 >> 4;
                 // (a tile that sums pieces has nothing to multiply: one round that hands the accumulator over)
                 for (int k0 = ti.kb0; (k0 < ti.kb1 || k0 == ti.kb0) && ok; k0 += C::kChunkBlocks) {
@@ -497,8 +500,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
 #pragma unroll
                             for (int term = 0; term < (kPlanes == 2 ? 3 : 1); ++term) {
                                 const uint64_t da = desc_k + slot + (kPlanes == 2 && term == 1 ? C::kPlaneBytes >> 4 : 0);
-                                const uint64_t db = desc_b0 + slot + (kRows128Bytes >> 4) +
-                                                    (kPlanes == 2 && term == 0 ? C::kPlaneBytes >> 4 : 0);
+                                const uint64_t db = desc_b0 + slot + (kPlanes == 2 && term == 0 ? C::kPlaneBytes >> 4 : 0);
 #pragma unroll
                                 for (int kk = 0; kk < BK / UMMA_K; ++kk)
                                     tcgen05_mma_bf16<kCtas>(tmem_d, da + kk * (32 >> 4), db + kk * step_b, idesc,
