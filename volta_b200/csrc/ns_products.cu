@@ -419,7 +419,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                 ok = false;
                 break;
             }
-            asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what other SMs stored
+            asm volatile("fence.proxy.async.global;" ::: "memory");  // TMA reads what other SMs stored
 #pragma unroll 1
             for (int kb = ti.kb0; kb < ti.kb1; ++kb) {
                 if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, wait_limit))) {
@@ -558,7 +558,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
                     ok = false;
                     break;
                 }
-                asm volatile("fence.proxy.async;" ::: "memory");
+                asm volatile("fence.proxy.async.global;" ::: "memory");
                 drain.fetch(0, 0);
                 drain.fetch(0, 1);
             }

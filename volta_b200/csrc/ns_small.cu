@@ -259,6 +259,28 @@ struct Image {
     }
 };
 
+// 8 elements of the input that lie in the image as they were
+template <int kPlanes>
+__device__ __forceinline__ void read_copied(int type, const Image &x, int i, int j, float (&u)[8])
+{
+    uint32_t q[kPlanes][4];
+#pragma unroll
+    for (int pl = 0; pl < kPlanes; ++pl) ld_shared_128(x.at(i, j) + pl * x.plane, q[pl][0], q[pl][1], q[pl][2], q[pl][3]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (kPlanes == 2) {
+#pragma unroll
+            for (int pl = 0; pl < kPlanes; ++pl) u[4 * pl + k] = __uint_as_float(q[pl][k]);
+        } else if (type == VB_DTYPE_BF16) {
+            u[2 * k] = __uint_as_float(q[0][k] << 16);
+            u[2 * k + 1] = __uint_as_float(q[0][k] & 0xffff0000u);
+        } else {
+            const float2 z = unpack_half(q[0][k]);
+            u[2 * k] = z.x, u[2 * k + 1] = z.y;
+        }
+    }
+}
+
 __device__ __forceinline__ void report(const NsError &error)
 {
     atomicExch(error.device, 4u);
@@ -305,11 +327,56 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
 
     // ---- the norm: every CTA of the cluster its columns, then all sums in rank order ----
     const Share s{d.n, d.m, rank * small.columns, small.columns, walks_i(a.a[kStep ? 1 : 0])};
+    // An input whose elements have as many bytes as the planes (16-bit types and one plane, f32 and two) is copied into
+    // the image as it is, all of it on its way at once, and summed and converted there; others are read twice.
+    const int type0 = w.types[0];
+    const bool copied = !kStep && (type0 == VB_DTYPE_F32) == (kPlanes == 2);
     double sum = 0.0;
-    for_u<kStep>(w, a, s, [&](int, int, int, const float (&)[8], const float (&u)[8]) {
+    if (copied) {
+        const NsArray &in = a.a[0];
+        for (int o = threadIdx.x; o < s.octets(); o += kThreads) {
+            int i, j, count;
+            s.locate(o, i, j, count);
+            const uint32_t to = x.at(i, j);
+            if (count == 8 && s.vec(in, a.direct & 1u)) {
+                const char *from = static_cast<const char *>(in.ptr) + s.offset(in, i, j) * (2 * kPlanes);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fma((double)u[e], (double)u[e], sum);
-    });
+                for (int pl = 0; pl < kPlanes; ++pl)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + pl * x.plane), "l"(from + pl * 16) : "memory");
+            } else {
+                float v[8];
+                load8(type0, in.ptr, s.offset(in, i, j), s.step(in), count, false, v);
+                if (kPlanes == 2) {
+#pragma unroll
+                    for (int pl = 0; pl < kPlanes; ++pl)
+                        st_shared_128(to + pl * x.plane, __float_as_uint(v[4 * pl]), __float_as_uint(v[4 * pl + 1]),
+                                      __float_as_uint(v[4 * pl + 2]), __float_as_uint(v[4 * pl + 3]));
+                } else {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {  // the input's own bits again
+                        if (type0 == VB_DTYPE_BF16) h[k] = __float_as_uint(v[2 * k]) >> 16 | (__float_as_uint(v[2 * k + 1]) & 0xffff0000u);
+                        else h[k] = pack_half(v[2 * k], v[2 * k + 1]);
+                    }
+                    st_shared_128(to, h[0], h[1], h[2], h[3]);
+                }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        for (int o = threadIdx.x; o < s.octets(); o += kThreads) {  // the octets this thread copied
+            int i, j, count;
+            s.locate(o, i, j, count);
+            float u[8];
+            read_copied<kPlanes>(type0, x, i, j, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fma((double)u[e], (double)u[e], sum);
+        }
+    } else {
+        for_u<kStep>(w, a, s, [&](int, int, int, const float (&)[8], const float (&u)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fma((double)u[e], (double)u[e], sum);
+        });
+    }
     sum = warp_sum(sum);
     if (lane == 0) sh.warp_sums[warp] = sum;
     tcgen05_fence_before();
@@ -333,8 +400,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     const float scale = isfinite(norm) ? (float)(ldexp(1.0, -shift) / (norm + (double)w.eps)) : nanf("");
 
     // ---- the share of X as f16 planes, blocks of 64 columns; step: the new velocity ----
-    for_u<kStep>(w, a, s, [&](int i, int j, int count, const float (&v)[8], const float (&u)[8]) {
-        if (kStep && !dead) s.write(w.types[1], a.a[1], a.direct & 2u, i, j, count, v);
+    auto put = [&](int i, int j, int count, const float (&u)[8]) {
         __half h[8], l[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -346,7 +412,21 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         const uint4 qh = *reinterpret_cast<const uint4 *>(h), ql = *reinterpret_cast<const uint4 *>(l);
         st_shared_128(at, qh.x, qh.y, qh.z, qh.w);
         if (kPlanes == 2) st_shared_128(at + x.plane, ql.x, ql.y, ql.z, ql.w);
-    });
+    };
+    if (copied) {
+        for (int o = threadIdx.x; o < s.octets(); o += kThreads) {
+            int i, j, count;
+            s.locate(o, i, j, count);
+            float u[8];
+            read_copied<kPlanes>(type0, x, i, j, u);
+            put(i, j, count, u);
+        }
+    } else {
+        for_u<kStep>(w, a, s, [&](int i, int j, int count, const float (&v)[8], const float (&u)[8]) {
+            if (kStep && !dead) s.write(w.types[1], a.a[1], a.direct & 2u, i, j, count, v);
+            put(i, j, count, u);
+        });
+    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
 
