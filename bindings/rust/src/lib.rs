@@ -28,6 +28,25 @@ pub mod ffi {
         _private: [u8; 0],
     }
 
+    #[repr(C)]
+    pub struct vb_ns_plan {
+        _private: [u8; 0],
+    }
+    #[repr(C)]
+    pub struct vb_ns_matrices {
+        _private: [u8; 0],
+    }
+
+    /// Scalars of `vb_muon_multi_tensor_step`.
+    #[repr(C)]
+    #[derive(Copy, Clone, Debug, Default)]
+    pub struct vb_muon_step_params {
+        pub lr: f32,
+        pub momentum: f32,
+        pub weight_decay: f32,
+        pub nesterov: i32,
+    }
+
     /// Same layout as `volta::gpu::OptimizerStepParams` (src/gpu/kernels.rs:42-54).
     #[repr(C)]
     #[derive(Copy, Clone, Debug, Default)]
@@ -46,6 +65,10 @@ pub mod ffi {
     pub const VB_NS_F32: c_int = 0;
     pub const VB_NS_BF16: c_int = 1;
     pub const VB_NS_F32_TC: c_int = 2;
+    pub const VB_NS_F16: c_int = 3;
+    pub const VB_DTYPE_F32: c_int = 0;
+    pub const VB_DTYPE_BF16: c_int = 1;
+    pub const VB_DTYPE_F16: c_int = 2;
     /// Flags of `vb_optimizer_step_ex`.
     pub const VB_STEP_DEFAULT: u32 = 0;
     pub const VB_STEP_NO_EXCHANGE: u32 = 1;
@@ -106,6 +129,25 @@ pub mod ffi {
             engine: *mut vb_engine, hp: *const vb_optimizer_step_params, n_tensors: i64, sizes: *const i64,
             params: *const *mut c_void, grads: *const *const c_void, state1: *const *mut c_void,
             state2: *const *mut c_void,
+        ) -> c_int;
+        // Newton-Schulz and Muon's step on device matrices the caller owns (src/nn/optim/muon.rs:50-163)
+        pub fn vb_ns_plan_create(
+            engine: *mut vb_engine, n_matrices: i64, rows: *const i64, cols: *const i64, n_steps: c_int,
+            coefficients: *const f32, eps: f32, ns_mode: c_int, out: *mut *mut vb_ns_plan,
+        ) -> c_int;
+        pub fn vb_ns_plan_destroy(plan: *mut vb_ns_plan) -> c_int;
+        pub fn vb_ns_plan_workspace(plan: *mut vb_ns_plan, bytes: *mut usize) -> c_int;
+        pub fn vb_ns_matrices_create(
+            plan: *mut vb_ns_plan, dtype: c_int, pointers: *const *mut c_void, strides: *const i64,
+            out: *mut *mut vb_ns_matrices,
+        ) -> c_int;
+        pub fn vb_ns_matrices_destroy(list: *mut vb_ns_matrices) -> c_int;
+        pub fn vb_orthogonalize(
+            plan: *mut vb_ns_plan, inputs: *const vb_ns_matrices, outputs: *const vb_ns_matrices,
+        ) -> c_int;
+        pub fn vb_muon_multi_tensor_step(
+            plan: *mut vb_ns_plan, hp: *const vb_muon_step_params, params: *const vb_ns_matrices,
+            grads: *const vb_ns_matrices, velocities: *const vb_ns_matrices, scales: *const f32,
         ) -> c_int;
     }
 }

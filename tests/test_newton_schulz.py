@@ -249,15 +249,17 @@ def test_orthogonalize_types_and_strides(engine, shape, layouts, kinds):
 
 
 @gpu
-def test_orthogonalize_in_place_zero_tiny_huge_and_undefined(engine):
+@pytest.mark.parametrize("mode", ["f16", "f32"])
+@pytest.mark.parametrize("shape", [(96, 160), (48, 100), (200, 30), (300, 70)])
+def test_orthogonalize_in_place_zero_tiny_huge_and_undefined(engine, shape, mode):
     import torch
     import volta_b200 as vb
-    shape = (96, 160)
+    ns_mode = vb.VB_NS_F32_TC if mode == "f32" else vb.VB_NS_F16
     base = _gradient(torch, shape, 1, torch.float32)
     xs = [torch.zeros(shape, device="cuda:0"), base * 1e-30, base * 1e30, base.clone(), base.clone(), base * 1e-9]
     xs[3][5, 7] = float("inf")
     xs[4][0, 0] = float("nan")
-    plan = vb.NewtonSchulzPlan([shape] * 6, QUINTIC, eps=1e-12, ns_mode=vb.VB_NS_F32_TC, engine=engine)
+    plan = vb.NewtonSchulzPlan([shape] * 6, QUINTIC, eps=1e-12, ns_mode=ns_mode, engine=engine)
     before = [x.clone() for x in xs]
     torch.cuda.synchronize()
     table = plan.matrices(xs)
@@ -269,8 +271,85 @@ def test_orthogonalize_in_place_zero_tiny_huge_and_undefined(engine):
     assert (xs[1].double() - want).abs().max().item() <= 2.0 ** -36
     for k, eps in ((2, 1e-12), (5, 1e-12)):
         want, bound = _exact(before[k].double(), QUINTIC, eps)
-        _close(xs[k], want, bound, _unit(vb.VB_NS_F32_TC, shape), torch.float32)
+        _close(xs[k], want, bound, _unit(ns_mode, shape), torch.float32)
     assert torch.isnan(xs[3]).all() and torch.isnan(xs[4]).all()
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["f16", "f32"])
+@pytest.mark.parametrize("coefficients", [QUINTIC[:1], [(2.0, -1.5, 0.5)] * 12, [(1.0, 0.0, 0.0)] * 2, [(1.5, -0.5, 0.0)] * 20],
+                         ids=["one", "twelve", "identity", "twenty linear"])
+def test_other_step_counts(engine, coefficients, mode):
+    import torch
+    import volta_b200 as vb
+    shapes = [(40, 90), (150, 150), (129, 700)]
+    ns_mode = vb.VB_NS_F32_TC if mode == "f32" else vb.VB_NS_F16
+    plan = vb.NewtonSchulzPlan(shapes, coefficients, ns_mode=ns_mode, engine=engine)
+    xs = [_gradient(torch, s, 20 + i, torch.float32) for i, s in enumerate(shapes)]
+    outs = [torch.empty_like(x) for x in xs]
+    torch.cuda.synchronize()
+    plan.orthogonalize(xs, outs)
+    engine.synchronize()
+    for x, o, s in zip(xs, outs, shapes):
+        want, bound = _exact(x.double(), coefficients)
+        _close(o, want, bound, _unit(ns_mode, s), torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["f16", "f32"])
+@pytest.mark.parametrize("shapes", [[(100, 4100)], [(4500, 128), (65, 2100)], [(20, 30)] * 210, [(70, 90)] * 130 + [(30, 9)] * 3,
+                                    [(512, 512)] * 40 + [(100, 700), (600, 1300), (1, 3)], [(64, 9000), (9000, 3)]],
+                         ids=["long", "tall", "many small", "many", "pairs", "very long"])
+def test_lists_of_every_kind(engine, shapes, mode):
+    """Contractions cut into pieces, several launches of small matrices, tile pairs with half-empty edges, columns
+    that do not fit one cluster."""
+    import torch
+    import volta_b200 as vb
+    ns_mode, dtype = (vb.VB_NS_F32_TC, torch.float32) if mode == "f32" else (vb.VB_NS_F16, torch.bfloat16)
+    plan = vb.NewtonSchulzPlan(shapes, QUINTIC, ns_mode=ns_mode, engine=engine)
+    xs = [_gradient(torch, s, 70 + i, dtype) for i, s in enumerate(shapes)]
+    outs = [torch.empty_like(x) for x in xs]
+    torch.cuda.synchronize()
+    plan.orthogonalize(xs, outs)
+    engine.synchronize()
+    for x, o, s in zip(xs, outs, shapes):
+        want, bound = _exact(x.double(), QUINTIC)
+        _close(o, want, bound, _unit(ns_mode, s), dtype)
+
+
+@gpu
+def test_offsets_beyond_32_bits(engine):
+    """Rows 1.1e9 elements apart: element offsets pass 2^31 in inputs, outputs, velocities and parameters."""
+    import torch
+    import volta_b200 as vb
+    pitch = 1_100_000_000
+    big = torch.zeros(3 * pitch, dtype=torch.bfloat16, device="cuda:0")
+    for shape, at in (((3, 40), 0), ((3, 40), pitch // 2)):
+        x = big.as_strided(shape, (pitch, 1), at)
+        x.copy_(_gradient(torch, shape, 4, torch.bfloat16))
+    wide = big.as_strided((3, 40), (pitch, 1), 0)
+    tall = big.as_strided((40, 3), (1, pitch), pitch // 2)
+    for x in (wide, tall):
+        plan = vb.NewtonSchulzPlan([x.shape], QUINTIC, engine=engine)
+        before = x.clone()
+        torch.cuda.synchronize()
+        plan.orthogonalize([x], [x])
+        engine.synchronize()
+        want, bound = _exact(before.double(), QUINTIC)
+        _close(x, want, bound, _unit(vb.VB_NS_F16, x.shape), torch.bfloat16)
+    # and through the general path: two rows of 130 columns, 130 rows of 70
+    plan = vb.NewtonSchulzPlan([(70, 130)], QUINTIC, engine=engine)
+    view = big.as_strided((70, 130), (40_000_000, 1), 0)
+    view.copy_(_gradient(torch, (70, 130), 6, torch.bfloat16))
+    before, velocity = view.clone(), torch.zeros(70, 130, device="cuda:0")
+    grad = _gradient(torch, (70, 130), 7, torch.bfloat16)
+    torch.cuda.synchronize()
+    plan.muon_step([view], [grad], [velocity], lr=0.1, momentum=0.0, nesterov=False)
+    engine.synchronize()
+    o, bound = _exact(grad.double(), QUINTIC)
+    want = before.double() - float(np.float32(0.1)) * o
+    off = torch.linalg.norm(view.double() - want).item()
+    assert off <= 0.1 * bound * _unit(vb.VB_NS_F16, (70, 130)) + 2.0 ** -8 * torch.linalg.norm(want).item()
 
 
 @gpu
@@ -514,28 +593,109 @@ def test_refusals(engine):
 
 
 @gpu
-def test_a_wait_that_runs_out_is_reported_and_stores_nothing():
+def test_producers_and_consumers_on_other_streams(engine):
+    """Inputs made on one stream, outputs read on another, ordered by events against the engine's stream."""
+    import torch
+    import volta_b200 as vb
+    shapes = [(60, 500), (256, 300)]
+    plan = vb.NewtonSchulzPlan(shapes, QUINTIC, engine=engine)
+    xs = [torch.empty(s, device="cuda:0") for s in shapes]
+    outs = [torch.empty(s, device="cuda:0") for s in shapes]
+    tx, to = plan.matrices(xs), plan.matrices(outs)
+    mine, producer, consumer = torch.cuda.ExternalStream(engine.stream), torch.cuda.Stream(), torch.cuda.Stream()
+    kept = []
+    torch.cuda.synchronize()
+    for seed in range(6):
+        with torch.cuda.stream(producer):
+            producer.wait_stream(mine)
+            for i, x in enumerate(xs):
+                x.copy_(_gradient(torch, shapes[i], 100 * seed + i, torch.float32))
+        mine.wait_stream(producer)
+        mine.wait_stream(consumer)
+        plan.orthogonalize(tx, to)
+        consumer.wait_stream(mine)
+        with torch.cuda.stream(consumer):
+            kept.append([o.clone() for o in outs])
+    torch.cuda.synchronize()
+    for seed in range(6):
+        for i, s in enumerate(shapes):
+            want, bound = _exact(_gradient(torch, s, 100 * seed + i, torch.float32).double(), QUINTIC)
+            _close(kept[seed][i], want, bound, _unit(vb.VB_NS_F16, s), torch.float32)
+
+
+@gpu
+def test_two_engines_at_once():
+    """Plans of two engines, each with launches that want the whole device, enqueued without waiting."""
+    import torch
+    import volta_b200 as vb
+    shapes = [(1024, 1024)] * 3 + [(64, 700)] * 5 + [(300, 1500)]
+    engines = [vb.Engine(0), vb.Engine(0)]
+    plans = [vb.NewtonSchulzPlan(shapes, QUINTIC, engine=e) for e in engines]
+    xs = [_gradient(torch, s, 3 + i, torch.bfloat16) for i, s in enumerate(shapes)]
+    outs = [[torch.empty_like(x) for x in xs] for _ in plans]
+    alone = [torch.empty_like(x) for x in xs]
+    torch.cuda.synchronize()
+    plans[0].orthogonalize(xs, alone)
+    engines[0].synchronize()
+    tables = [(p.matrices(xs), p.matrices(o)) for p, o in zip(plans, outs)]
+    for _ in range(5):
+        for p, t in zip(plans, tables):
+            p.orthogonalize(*t)
+    for e in engines:
+        e.synchronize()
+    for o in outs:
+        assert all(torch.equal(a, b) for a, b in zip(o, alone))
+    for p in plans:
+        p.close()
+    for e in engines:
+        e.close()
+
+
+@gpu
+def test_engine_gone_and_workspace_refused():
+    import torch
+    import volta_b200 as vb
+    eng = vb.Engine(0)
+    with pytest.raises(vb.VoltaB200Error, match="workspace"):
+        vb.NewtonSchulzPlan([(65536, 65536)] * 4, QUINTIC[:2], engine=eng)  # 240 GB
+    plan = vb.NewtonSchulzPlan([(70, 80)], QUINTIC, engine=eng)
+    x, o = torch.ones(70, 80, device="cuda:0"), torch.zeros(70, 80, device="cuda:0")
+    plan.orthogonalize([x], [o])
+    eng.synchronize()
+    assert o.abs().max().item() > 0
+    eng.close()
+    with pytest.raises(vb.VoltaB200Error, match="destroyed"):
+        plan.orthogonalize([x], [o])
+    plan.close()
+    with pytest.raises(vb.VoltaB200Error, match="null"):
+        plan.orthogonalize([x], [o])
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [[(300, 400)], [(50, 400)], [(50, 400), (300, 400)]])
+def test_a_wait_that_runs_out_is_reported_and_stores_nothing(shapes):
     import torch
     import volta_b200 as vb
     from volta_b200 import _lib
     eng = vb.Engine(0)
-    plan = vb.NewtonSchulzPlan([(300, 400)], QUINTIC, engine=eng)
-    x = _gradient(torch, (300, 400), 1, torch.float32)
-    out = torch.full_like(x, 3.0)
+    plan = vb.NewtonSchulzPlan(shapes, QUINTIC, engine=eng)
+    xs = [_gradient(torch, s, 1, torch.float32) for s in shapes]
+    outs = [torch.full_like(x, 3.0) for x in xs]
     torch.cuda.synchronize()
     _lib.call("vb_debug_ns_plan_withhold_loads", plan._h, 2000)
-    plan.orthogonalize([x], [out])
+    plan.orthogonalize(xs, outs)
     with pytest.raises(vb.VoltaB200Error) as e:
         eng.synchronize()
     assert e.value.status == 4
-    assert (out == 3.0).all()
+    if len(shapes) == 1:  # of two launches side by side only the first one's waits run out
+        assert (outs[0] == 3.0).all()
     with pytest.raises(vb.VoltaB200Error) as e:
-        plan.orthogonalize([x], [out])
+        plan.orthogonalize(xs, outs)
     assert e.value.status == 4
     plan.close()
-    fresh = vb.NewtonSchulzPlan([(300, 400)], QUINTIC, engine=eng)  # the engine stays usable
-    fresh.orthogonalize([x], [out])
+    fresh = vb.NewtonSchulzPlan(shapes, QUINTIC, engine=eng)  # the engine stays usable
+    fresh.orthogonalize(xs, outs)
     eng.synchronize()
-    assert not (out == 3.0).any()
+    assert not any((o == 3.0).any() for o in outs)
     fresh.close()
     eng.close()

@@ -624,7 +624,12 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         }
         if (round == 0) {
             p->workspace = c.used;
-            VB_CUDA(cudaMalloc((void **)&p->d_base, std::max<size_t>(c.used, 1024)));
+            const cudaError_t err = cudaMalloc((void **)&p->d_base, std::max<size_t>(c.used, 1024));
+            if (err != cudaSuccess) {
+                cudaGetLastError();  // nothing of it is left for the checks after later launches
+                p->d_base = nullptr;
+                return fail(VB_ERR_CUDA, "the plan's workspace of %zu bytes could not be allocated: %s", c.used, cudaGetErrorString(err));
+            }
         } else {
             if (!small.empty()) {
                 VB_CUDA(cudaMemcpyAsync(d_small, small.data(), small.size() * sizeof(NsSmallMatrix), cudaMemcpyHostToDevice, p->eng->stream));
