@@ -201,8 +201,8 @@ int read_steps(int n_steps, const float *coefficients, std::vector<Step> *steps)
 GroupLimits group_limits(int64_t rows, int64_t cols, int planes, bool small)
 {
     const double n = (double)std::min(rows, cols), m = (double)std::max(rows, cols);
-    if (small && planes == 1) return {5e4, 2e4};
-    if (small) return {75.0 * std::sqrt(n / 64.0), 17.0};
+    if (small && planes == 1) return {5e4 * std::sqrt(n / 64.0), 2e4 * std::sqrt(n / 64.0)};
+    if (small) return {75.0 * std::sqrt(n / 64.0), 17.0 * std::min(1.0, std::sqrt(n / 32.0))};
     if (2.0 * m < 3.0 * n) return {0.0, 0.0};
     return {150.0 * std::min(1.0, std::sqrt(n / 256.0)), 17.0};
 }
@@ -502,6 +502,9 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         NsSmallOp *d_small_ops = c.take<NsSmallOp>(small_ops.size());
         p->small.matrices = d_small;
         p->small.ops = d_small_ops;
+        double *d_coefficients = c.take<double>(3 * steps.size());
+        p->small.coefficients = d_coefficients;
+        p->small.n_steps = (int)steps.size();
         p->d_tile_matrix = d_tile_matrix;
         problems.clear();
         std::vector<size_t> stage_begin;  // of every stage's products in `problems`
@@ -632,6 +635,8 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             }
         } else {
             if (!small.empty()) {
+                static_assert(sizeof(Step) == 3 * sizeof(double), "copied as a, b, c");
+                VB_CUDA(cudaMemcpyAsync(d_coefficients, steps.data(), steps.size() * sizeof(Step), cudaMemcpyHostToDevice, p->eng->stream));
                 VB_CUDA(cudaMemcpyAsync(d_small, small.data(), small.size() * sizeof(NsSmallMatrix), cudaMemcpyHostToDevice, p->eng->stream));
                 VB_CUDA(cudaMemcpyAsync(d_small_ops, small_ops.data(), small_ops.size() * sizeof(NsSmallOp), cudaMemcpyHostToDevice, p->eng->stream));
             }

@@ -138,6 +138,7 @@ int launch_ns_finish(const NsElementwise &w, const NsBatchArgs &b, const int32_t
 
 // ---- matrices with a short side of at most 64 (ns_small.cu) ----------------------------------
 constexpr int kNsSmallSide = 64;
+constexpr int kNsTinySide = 16;      // up to here VB_NS_F32_TC keeps the short side in f64
 constexpr int kNsSmallOps = 128;     // longest program
 constexpr int kNsSmallSquares = 5;
 constexpr int kNsSmallCluster = 8;   // most CTAs of one matrix
@@ -157,6 +158,8 @@ struct NsSmallMatrix {
 struct NsSmall {
     const NsSmallMatrix *matrices;  // of a whole plan
     const NsSmallOp *ops;
+    const double *coefficients;     // a, b, c of every step
+    int n_steps;
     int cluster;                    // CTAs per matrix
     int columns;                    // columns of X per CTA, a multiple of 64
 };

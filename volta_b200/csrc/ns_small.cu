@@ -16,6 +16,10 @@
 // What a stage costs (cycles, 64 x 288 to f32 accuracy): 12 MMAs 400, their completion 250, tensor memory to
 // shared memory 600, barriers 200.
 //
+// A short side of at most 16 to f32 accuracy (tiny) is worked on in f64 on the CUDA cores instead: planes of 22
+// bits, amplified by steep coefficients, left errors of 1e-5 to 2e-5 at 8 x 3000, and 16 x 16 products are nothing.
+// U stays in shared memory in f32; G, the polynomial of G and its product with U are f64.
+//
 // Shared memory: five squares of 16 KiB, the share of X, and 8 KiB that M = 128 operands run over into (rows
 // 64 .. 127 of A are whatever lies there; they only reach rows of the accumulator that nobody reads).
 #include <algorithm>
@@ -35,6 +39,13 @@ constexpr int kSquareBytes = 2 * kBlockBytes;     // two planes
 constexpr int kSquaresBytes = kNsSmallSquares * kSquareBytes;
 constexpr int kTmemCols = 256;
 constexpr int kSumSquare = kNsSmallSquares - 1;   // the square whose memory holds partial Grams (f32) between stages
+
+constexpr int kTiny = kNsTinySide;
+struct TinySquares {  // in the squares' memory
+    double g[kTiny][kTiny + 1], q[kTiny][kTiny + 1], t[kTiny][kTiny + 1], p[kTiny][kTiny + 1];
+    double part[2][kTiny * kTiny];  // this CTA's Gram, by halves of its columns
+};
+static_assert(sizeof(TinySquares) <= kSquaresBytes, "they share memory");
 
 struct alignas(8) Shared {
     uint64_t done;
@@ -281,6 +292,77 @@ __device__ __forceinline__ void read_copied(int type, const Image &x, int i, int
     }
 }
 
+// Element (i, j) of U where the image holds f32: 8 along the image's rows are 4 in plane 0 and 4 in plane 1.
+__device__ __forceinline__ float tiny_u(const Image &x, int i, int j)
+{
+    const int along = x.turned ? i : j, first = along & ~7;
+    const uint32_t at = (x.turned ? x.at(first, j) : x.at(i, first)) + ((along & 4) ? x.plane : 0u) + (uint32_t)(along & 3) * 4u;
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+// ts.p <- the polynomial of the Gram, over (|U|_F + eps): O = ts.p U.  Every CTA of the cluster computes it from the same sums.
+__device__ __forceinline__ void tiny_polynomial(TinySquares &ts, const NsSmall &small, const Share &s, const Image &x, int clusters,
+                                                double scale, uint32_t smem_ts)
+{
+    const int pair = (int)threadIdx.x & (kTiny * kTiny - 1), half = (int)threadIdx.x / (kTiny * kTiny);
+    const int r = pair / kTiny, c = pair % kTiny;
+    static_assert(kThreads == 2 * kTiny * kTiny, "a thread per element and half of the columns");
+    double sum = 0.0;
+    const int columns = s.columns / 2;
+    for (int j = half * columns; j < (half + 1) * columns; ++j)
+        sum = fma((double)tiny_u(x, r, j), (double)tiny_u(x, c, j), sum);
+    ts.part[half][pair] = sum;
+    cluster_sync_all();
+    if (half == 0) {
+        double g = 0.0;
+        for (int k = 0; k < clusters; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                g += ld_cluster_f64(map_to_cta(smem_ts + (uint32_t)((const char *)&ts.part[h][pair] - (const char *)&ts), (uint32_t)k));
+        ts.g[r][c] = g / scale / scale;
+        ts.p[r][c] = r == c ? 1.0 / scale : 0.0;
+    }
+    cluster_sync_all();
+    auto product = [&](const double (&a)[kTiny][kTiny + 1], const double (&b)[kTiny][kTiny + 1]) {
+        double v = 0.0;
+#pragma unroll
+        for (int k = 0; k < kTiny; ++k) v = fma(a[r][k], b[k][c], v);
+        return v;
+    };
+    for (int k = 0; k < small.n_steps; ++k) {
+        const double sa = small.coefficients[3 * k], sb = small.coefficients[3 * k + 1], sc = small.coefficients[3 * k + 2];
+        if (half == 0) ts.q[r][c] = (r == c ? sa : 0.0) + sb * ts.g[r][c] + sc * product(ts.g, ts.g);
+        __syncthreads();
+        const double next_p = half == 0 ? product(ts.q, ts.p) : 0.0;
+        if (half == 1) ts.t[r][c] = product(ts.q, ts.g);
+        __syncthreads();
+        if (half == 0) ts.p[r][c] = next_p;
+        if (half == 1) ts.g[r][c] = product(ts.t, ts.q);
+        __syncthreads();
+    }
+}
+// 8 elements of P U along i or along j
+__device__ __forceinline__ void tiny_output(const TinySquares &ts, const Image &x, int n, bool along_i, int i, int j, float (&f)[8])
+{
+    double v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0;
+    for (int k = 0; k < n; ++k) {
+        if (along_i) {
+            const double u = (double)tiny_u(x, k, j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = fma(ts.p[min(i + e, kTiny - 1)][k], u, v[e]);
+        } else {
+            const double p = ts.p[i][k];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = fma(p, (double)tiny_u(x, k, j + e), v[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+}
+
 __device__ __forceinline__ void report(const NsError &error)
 {
     atomicExch(error.device, 4u);
@@ -400,7 +482,16 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     const float scale = isfinite(norm) ? (float)(ldexp(1.0, -shift) / (norm + (double)w.eps)) : nanf("");
 
     // ---- the share of X as f16 planes, blocks of 64 columns; step: the new velocity ----
+    const bool tiny = kPlanes == 2 && d.n <= kTiny;
     auto put = [&](int i, int j, int count, const float (&u)[8]) {
+        if (tiny) {  // as it is
+            const uint32_t to = x.at(i, j);
+#pragma unroll
+            for (int pl = 0; pl < kPlanes; ++pl)
+                st_shared_128(to + pl * x.plane, __float_as_uint(u[4 * pl]), __float_as_uint(u[4 * pl + 1]),
+                              __float_as_uint(u[4 * pl + 2]), __float_as_uint(u[4 * pl + 3]));
+            return;
+        }
         __half h[8], l[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -413,7 +504,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         st_shared_128(at, qh.x, qh.y, qh.z, qh.w);
         if (kPlanes == 2) st_shared_128(at + x.plane, ql.x, ql.y, ql.z, ql.w);
     };
-    if (copied) {
+    if (copied && !tiny) {
         for (int o = threadIdx.x; o < s.octets(); o += kThreads) {
             int i, j, count;
             s.locate(o, i, j, count);
@@ -421,7 +512,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
             read_copied<kPlanes>(type0, x, i, j, u);
             put(i, j, count, u);
         }
-    } else {
+    } else if (!copied) {
         for_u<kStep>(w, a, s, [&](int i, int j, int count, const float (&v)[8], const float (&u)[8]) {
             if (kStep && !dead) s.write(w.types[1], a.a[1], a.direct & 2u, i, j, count, v);
             put(i, j, count, u);
@@ -457,7 +548,9 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
     auto square = [&](int k) { return squares + (uint32_t)(k * kSquareBytes); };
     auto square_operand = [&](int k) { return desc.operand(square(k), kBlockBytes, false); };
 
-    for (int op0 = 0; op0 < d.n_ops;) {
+    TinySquares &ts = *reinterpret_cast<TinySquares *>(smem);
+    if (tiny) tiny_polynomial(ts, small, s, x, clusters, norm + (double)w.eps, squares);
+    for (int op0 = tiny ? d.n_ops : 0; op0 < d.n_ops;) {
         const NsSmallOp first = sh.ops[op0];
         if (first.kind == 1) {
             // ---- Gram: this CTA's columns, then the cluster's sum ----
@@ -609,7 +702,7 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
         const NsArray &dst = a.a[kOut];
         Share out = s;
         out.along_i = walks_i(dst);
-        const float rate = w.rate * a.scale;
+        const float rate = w.rate * a.scale, final_scale = tiny ? 1.0f : d.final_scale;
         for (int o0 = threadIdx.x; o0 < out.octets(); o0 += kThreads * kInFlight) {
             Raw p[kStep ? kInFlight : 1];
 #pragma unroll
@@ -628,8 +721,10 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                 float f[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+                if (tiny) tiny_output(ts, x, d.n, out.along_i, i, j, f);
 #pragma unroll
                 for (int pl = 0; pl < kPlanes; ++pl) {
+                    if (tiny) break;
                     if (out.along_i == x.turned) {
                         uint32_t v[4];
                         ld_shared_128(x.at(i, j) + pl * x.plane, v[0], v[1], v[2], v[3]);
@@ -652,10 +747,10 @@ ns_small_kernel(const NsElementwise w, const NsSmall small, const __grid_constan
                     float pp[8];
                     p[kStep ? k : 0].get(w.types[kOut], dst.ptr, out.offset(dst, i, j), out.step(dst), count, pp);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = fmaf(-rate, f[e] * d.final_scale, pp[e] * w.decay);
+                    for (int e = 0; e < 8; ++e) f[e] = fmaf(-rate, f[e] * final_scale, pp[e] * w.decay);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= d.final_scale;
+                    for (int e = 0; e < 8; ++e) f[e] *= final_scale;
                 }
                 out.write(w.types[kOut], dst, (a.direct >> kOut) & 1u, i, j, count, f);
             }
