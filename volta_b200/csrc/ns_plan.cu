@@ -24,6 +24,7 @@
 #include <cmath>
 
 #include <algorithm>
+#include <map>
 #include <memory>
 #include <numeric>
 
@@ -397,6 +398,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
     const int64_t n = p->n;
     std::vector<Schedule> schedules;       // the different ones among the matrices
     std::vector<std::vector<std::vector<int>>> groupings;
+    std::map<std::pair<double, double>, size_t> by_limits;
     std::vector<std::vector<NsSmallOp>> programs;
     std::vector<size_t> kind((size_t)n);
     std::vector<NsSmallMatrix> small;
@@ -415,9 +417,15 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         if (d.n == 0) d.m = 0;
         const auto limits = [&](bool as_small) { return group_limits(d.n, d.m, p->planes, as_small); };
         auto find = [&](const GroupLimits &l, size_t *which) -> int {
+            const auto known = by_limits.find({l.first, l.later});
+            if (known != by_limits.end()) {
+                *which = known->second;
+                return VB_OK;
+            }
             const auto groups = make_groups(steps, l);
             *which = 0;
             while (*which < groupings.size() && groupings[*which] != groups) ++*which;
+            by_limits[{l.first, l.later}] = *which;
             if (*which < groupings.size()) return VB_OK;
             groupings.push_back(groups);
             schedules.emplace_back();

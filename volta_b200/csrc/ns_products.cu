@@ -65,16 +65,22 @@ constexpr int kFirstEpiWarp = 2;  // warp 0 produces, warp 1 issues
 constexpr int kThreads = (kFirstEpiWarp + kEpiWarps) * 32;
 constexpr int kPieceCols = 64;
 constexpr int kPieceBytes = 32 * kPieceCols * 2;  // 32 rows of 128 bytes, 16-byte parts of row r at part ^ (r & 7)
-constexpr int kEpiWarpBytes = 3 * kPieceBytes;    // term, result, mirrored result or a second term
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 5;
+constexpr int kSmemBytes = 232448 - 2048;  // 227 KiB less alignment and barriers
 
 template <int kCtas, int kPlanes>
 struct Cfg {
     static constexpr int BN = kCtas == 2 && kPlanes == 1 ? 256 : 128;  // columns of a tile
     static constexpr int kBRows = BN / kCtas;                           // rows of B a CTA stages
-    static constexpr int kStages = kPlanes == 1 ? 4 : 2;
     static constexpr int kPlaneBytes = kRows128Bytes + kBRows * BK * 2;  // 128 rows of A, kBRows of B
     static constexpr int kStageBytes = kPlanes * kPlaneBytes;
+    // An epilogue warp's buffers: a term, a second term or the mirrored result, and, where it has more pieces than one
+    // per tile (so that the next term arrives while a result leaves), a separate one for the result.
+    static constexpr int kEpiBuffers = BN / 2 > kPieceCols ? 3 : 2;
+    static constexpr int kEpiWarpBytes = kEpiBuffers * kPieceBytes;
+    static constexpr int kStages = (kSmemBytes - kEpiWarps * kEpiWarpBytes) / kStageBytes < kMaxStages
+                                       ? (kSmemBytes - kEpiWarps * kEpiWarpBytes) / kStageBytes
+                                       : kMaxStages;
     static constexpr int kTmemCols = 2 * BN;
     static constexpr int kChunkBlocks = kPlanes == 1 ? 1 << 20 : 128 / BK;  // k blocks one accumulator takes
 };
@@ -93,7 +99,7 @@ template <int kCtas, int kPlanes>
 constexpr size_t smem_bytes()
 {
     using C = Cfg<kCtas, kPlanes>;
-    return 1024 + (size_t)C::kStages * C::kStageBytes + kEpiWarps * kEpiWarpBytes + sizeof(Barriers);
+    return 1024 + (size_t)C::kStages * C::kStageBytes + kEpiWarps * C::kEpiWarpBytes + sizeof(Barriers);
 }
 static_assert(smem_bytes<2, 1>() <= 232448 && smem_bytes<1, 2>() <= 232448, "a CTA has 227 KiB of shared memory");
 
@@ -216,6 +222,8 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 // The warp's share of one tile: kCols columns of 32 rows.
 template <int kPlanes, int kCols>
 struct Drain {
+    static constexpr int kResult = kCols > kPieceCols ? kPieceBytes : 0;  // offsets of the buffers
+    static constexpr int kMirror = kResult + kPieceBytes;
     const NsProduct *p;
     uint8_t *buffers;     // this warp's
     uint64_t *term_full;  // this warp's two barriers
@@ -231,7 +239,7 @@ struct Drain {
         if (lane != 0 || r >= per_piece || piece >= kCols / kPieceCols) return;
         uint64_t *full = term_full + (r & 1);
         mbar_expect_tx(full, kPieceBytes);
-        tma_load_2d<1>(buffers + (r & 1) * 2 * kPieceBytes, &p->map_term[r / kPlanes], col0 + piece * kPieceCols,
+        tma_load_2d<1>(buffers + (r & 1) * kMirror, &p->map_term[r / kPlanes], col0 + piece * kPieceCols,
                        row0 + (r % kPlanes) * p->plane_rows, smem_u32(full));
     }
     // one plane of a finished piece: h[k] holds columns 2k and 2k + 1 of this lane's row
@@ -239,11 +247,11 @@ struct Drain {
     {
         if (lane == 0) bulk_wait_read();  // the stores before this one have left the buffers
         __syncwarp();
-        const uint32_t out = smem_u32(buffers) + kPieceBytes, row = out + (uint32_t)(lane * 128);
+        const uint32_t out = smem_u32(buffers) + kResult, row = out + (uint32_t)(lane * 128);
 #pragma unroll
         for (int q = 0; q < 8; ++q)
             st_shared_128(row + (uint32_t)((q ^ (lane & 7)) << 4), h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
-        const uint32_t turned = out + kPieceBytes;
+        const uint32_t turned = smem_u32(buffers) + kMirror;
         if (mirror) {
             // column 2k (even lanes) or 2k + 1 (odd lanes), rows of a pair of lanes: 32 words of two 64-byte rows
             const uint32_t word = turned + (uint32_t)((lane & 1) * 64 + (lane >> 1) * 4);
@@ -291,7 +299,7 @@ struct Drain {
                 if (!__all_sync(0xffffffffu, mbar_wait(term_full + buf, (term_phase >> buf) & 1u, abort_flag, wait_limit))) return false;
                 term_phase ^= 1u << buf;
                 const float c = p->term[r / kPlanes] * mult;
-                const uint32_t row = smem_u32(buffers) + (uint32_t)(buf * 2 * kPieceBytes + lane * 128);
+                const uint32_t row = smem_u32(buffers) + (uint32_t)(buf * kMirror + lane * 128);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     uint32_t w[4];
@@ -345,7 +353,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *epi_stage = smem + (size_t)C::kStages * C::kStageBytes;
-    Barriers *bars = reinterpret_cast<Barriers *>(epi_stage + kEpiWarps * kEpiWarpBytes);
+    Barriers *bars = reinterpret_cast<Barriers *>(epi_stage + kEpiWarps * C::kEpiWarpBytes);
     volatile uint32_t *abort_flag = &bars->abort;
 
     const int warp = uniform((int)(threadIdx.x >> 5));
@@ -526,7 +534,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         // ---- epilogue: warp w reads TMEM lane quarter w % 4 and half of the columns ----
         constexpr int kCols = C::BN / 2;
         const int quarter = warp & 3, col_half = (warp - kFirstEpiWarp) >> 2;
-        uint8_t *const my_buffers = epi_stage + (size_t)(warp - kFirstEpiWarp) * kEpiWarpBytes;
+        uint8_t *const my_buffers = epi_stage + (size_t)(warp - kFirstEpiWarp) * C::kEpiWarpBytes;
         uint64_t *const term_full = &bars->term_full[2 * (warp - kFirstEpiWarp)];
         uint32_t term_phase = 0;
         int acc = 0;
