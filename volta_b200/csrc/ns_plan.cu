@@ -25,8 +25,10 @@
 
 #include <algorithm>
 #include <map>
+#include <functional>
 #include <memory>
 #include <numeric>
+#include <queue>
 
 #include "engine.h"
 #include "ns_plan.h"
@@ -364,13 +366,15 @@ int gram_parts(const NsProduct &pr, int shape, uint32_t stage_tiles, int sm_coun
     return std::max(1, std::min(pr.K / kNsKBlock / 8, sm_count / (int)stage_tiles));
 }
 
+constexpr double kTileCycles[2][2] = {{11.9, 10.5}, {18.4, 18.7}};  // per element of the contraction: [planes - 1][shape]
+
 // The shape whose stages take less time if every stage is waited for: whole rounds of tiles over the device's
 // CTAs (pairs), at the measured cycles of a tile per element of the contraction, plus what a stage costs
 // besides (signals, first loads, epilogue: about 12000 cycles).  One plane: a 128 x 128 tile takes 10.5 cycles
 // (issue bound), a pair's 256 x 256 one 11.9 (bound by L2); two planes 18.7 and, 256 x 128, 18.4.
 int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t> &stage_begin, int planes, int sm_count)
 {
-    const double cycles[2][2] = {{11.9, 10.5}, {18.4, 18.7}}, per_stage = 12000.0;
+    const double per_stage = 12000.0;
     double cost[2] = {0.0, 0.0};
     for (int shape = 0; shape < 2; ++shape) {
         const double groups = shape == NS_TILE_PAIR ? sm_count / 2 : sm_count;
@@ -387,10 +391,78 @@ int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t>
             }
             if (tiles == 0) continue;
             const double rounds = std::ceil(tiles / groups), mean = work / tiles;
-            cost[shape] += per_stage * (cut ? 2 : 1) + cycles[planes - 1][shape] * std::max(longest, cut ? work / groups : rounds * mean);
+            cost[shape] += per_stage * (cut ? 2 : 1) + kTileCycles[planes - 1][shape] * std::max(longest, cut ? work / groups : rounds * mean);
         }
     }
     return cost[NS_TILE_PAIR] <= cost[NS_TILE_128] ? NS_TILE_PAIR : NS_TILE_128;
+}
+
+// Deals the tiles out to the groups: the device is played through with the measured cost of a tile (see pick_shape), a
+// free group takes a tile of the matrix that has the longest way to go among those whose last stage is stored by
+// then.  So a long contraction of one matrix does not hold up the stages of the others, as it does where tiles are dealt
+// round robin (one d = 1024 transformer layer: 320 us).  A stage is dealt after the one before it: every group's
+// list follows the order of dealing, in which a tile comes after those it waits for.
+void deal_tiles(const std::vector<NsTile> &tiles, const std::vector<NsProduct> &problems, int64_t n_matrices, double cycles_per_k,
+                int groups, std::vector<NsTile> *dealt, std::vector<int32_t> *begin)
+{
+    const double epilogue = 6000.0, signal = 3000.0;
+    struct Matrix {
+        std::vector<std::vector<int32_t>> stages;  // tiles that wait for the same earlier ones
+        std::vector<double> way;                   // from the start of a stage to the end
+        size_t stage = 0, next = 0;
+        double stored = 0.0, ready = 0.0;  // the stage's last tile; the one before's
+    };
+    std::vector<Matrix> ms((size_t)n_matrices);
+    auto cost = [&](int32_t t) { return cycles_per_k * kNsKBlock * (tiles[(size_t)t].kb1 - tiles[(size_t)t].kb0); };
+    for (int32_t t = 0; t < (int32_t)tiles.size(); ++t) {
+        Matrix &m = ms[(size_t)problems[(size_t)tiles[(size_t)t].problem].matrix];
+        if (m.stages.empty() || tiles[(size_t)m.stages.back().front()].after != tiles[(size_t)t].after) m.stages.emplace_back();
+        m.stages.back().push_back(t);
+    }
+    using Event = std::pair<double, int64_t>;
+    std::priority_queue<Event, std::vector<Event>, std::greater<Event>> free, waiting;  // (time, group) and (time, matrix)
+    std::priority_queue<Event> ready;                                                    // (way to go, matrix)
+    for (int64_t i = 0; i < n_matrices; ++i) {
+        Matrix &m = ms[(size_t)i];
+        m.way.assign(m.stages.size() + 1, 0.0);
+        for (size_t k = m.stages.size(); k-- > 0;) {
+            double longest = 0.0, sum = 0.0;
+            for (int32_t t : m.stages[k]) longest = std::max(longest, cost(t)), sum += cost(t);
+            m.way[k] = m.way[k + 1] + std::max(longest, sum / groups) + epilogue + signal;
+        }
+        if (!m.stages.empty()) waiting.push({0.0, i});
+    }
+    for (int64_t g = 0; g < groups; ++g) free.push({0.0, g});
+    std::vector<std::vector<int32_t>> lists((size_t)groups);
+    for (size_t left = tiles.size(); left > 0; --left) {
+        auto [now, g] = free.top();
+        free.pop();
+        if (ready.empty()) now = std::max(now, waiting.top().first);
+        while (!waiting.empty() && waiting.top().first <= now) {
+            const int64_t i = waiting.top().second;
+            waiting.pop();
+            ready.push({ms[(size_t)i].way[ms[(size_t)i].stage], i});
+        }
+        const int64_t i = ready.top().second;
+        Matrix &m = ms[(size_t)i];
+        const int32_t t = m.stages[m.stage][m.next++];
+        lists[(size_t)g].push_back(t);
+        now = std::max(now, m.ready);
+        free.push({now + std::max(cost(t), epilogue), g});
+        m.stored = std::max(m.stored, now + cost(t) + epilogue + signal);
+        if (m.next == m.stages[m.stage].size()) {
+            ready.pop();
+            m.next = 0;
+            m.ready = m.stored;
+            if (++m.stage < m.stages.size()) waiting.push({m.stored, i});
+        }
+    }
+    dealt->clear();
+    begin->assign(1, 0);
+    for (const auto &list : lists) {
+        for (int32_t t : list) dealt->push_back(tiles[(size_t)t]);
+        begin->push_back((int32_t)dealt->size());
+    }
 }
 
 int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
@@ -617,8 +689,20 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         NsProduct *d_problems = c.take<NsProduct>(problems.size());
         NsTile *d_tiles = c.take<NsTile>(tile_list.size());
         if (tile_list.size() > (size_t)INT32_MAX) return fail(VB_ERR_UNSUPPORTED, "the plan's products have too many tiles");
-        // more CTAs (pairs) than the largest stage has tiles would mostly wait, on SMs that others could use
-        p->products = {d_problems, d_tiles, p->ew.stored, partials, (int)tile_list.size(), (int)widest};
+        // more groups than the largest stage has tiles would mostly wait, on SMs that others could use
+        int groups = 0;
+        VB_TRY(ns_resident_groups(p->shape, p->planes, p->eng->sm_count, &groups));
+        groups = std::max(1, std::min(groups, (int)widest));
+        int32_t *d_begin = c.take<int32_t>((size_t)groups + 1);
+        p->products = {d_problems, d_tiles, d_begin, p->ew.stored, partials, (int)tile_list.size(), groups};
+        std::vector<int32_t> begin;
+        if (round == 1) {
+            std::vector<NsTile> dealt;
+            deal_tiles(tile_list, problems, n, kTileCycles[p->planes - 1][p->shape], groups, &dealt, &begin);
+            tile_list.swap(dealt);
+            VB_CUDA(cudaMemcpyAsync(d_begin, begin.data(), begin.size() * sizeof(int32_t), cudaMemcpyHostToDevice, p->eng->stream));
+            VB_CUDA(cudaStreamSynchronize(p->eng->stream));  // `begin` goes out of scope
+        }
         if (round == 1) {
             VB_CUDA(cudaMemcpyAsync(d_problems, problems.data(), problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
@@ -709,7 +793,7 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, bool turned, Fill
     prof_end(e, VB_PHASE_MUON_PRE);
     if (p->products.n_tiles > 0) {
         prof_begin(e, VB_PHASE_MUON_NS);
-        VB_TRY(launch_ns_products(p->products, p->shape, p->planes, w.active, p->error, e->sm_count, e->stream, wait_limit, p->withhold));
+        VB_TRY(launch_ns_products(p->products, p->shape, p->planes, w.active, p->error, e->stream, wait_limit, p->withhold));
         e->launches += 1;
         p->withhold = false;
         prof_end(e, VB_PHASE_MUON_NS);

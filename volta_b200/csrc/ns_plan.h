@@ -55,14 +55,16 @@ struct NsTile {
     int32_t part, parts;
 };
 
-// The tiles of every stage of every matrix, earlier stages first.
+// The tiles of every stage of every matrix, CTA (pair) by CTA (pair): group g takes tiles begin[g] .. begin[g + 1] - 1 in
+// order.  The orders are consistent with one order of all tiles in which every tile follows those it waits for.
 struct NsLaunch {
     const NsProduct *problems;
     const NsTile *tiles;
+    const int32_t *begin;
     uint32_t *stored;  // per matrix: epilogue warps' arrivals, zeroed by the gather pass
     float *partials;   // slots of 128 x 128
     int n_tiles;
-    int widest;        // tiles of the largest stage
+    int groups;
 };
 
 // Tile shapes of the product kernel.
@@ -70,6 +72,7 @@ enum NsTileShape {
     NS_TILE_PAIR = 0,  // two CTAs, 256 x 256 (two planes: 256 x 128)
     NS_TILE_128 = 1    // one CTA, 128 x 128
 };
+int ns_resident_groups(int shape, int planes, int sm_count, int *groups);  // CTAs (pairs) the device holds at once
 void ns_tile_extent(int shape, int planes, int *bm, int *bn);
 // Where a kernel reports a wait that ran out: a device word later kernels look at, a mapped one for the host.
 struct NsError {
@@ -77,7 +80,7 @@ struct NsError {
 };
 // withhold: test hook, the producers stage nothing so that every wait runs out
 int launch_ns_products(const NsLaunch &launch, int shape, int planes, const uint32_t *d_active, NsError error,
-                       int sm_count, cudaStream_t stream, uint32_t wait_limit, bool withhold);
+                       cudaStream_t stream, uint32_t wait_limit, bool withhold);
 // A row-major f16 matrix [outer][inner] as the kernel moves it.
 enum NsMap {
     NS_MAP_ROWS = 0,   // 64 x 128 boxes, 128-byte swizzle: 128 rows x 64 k of an operand

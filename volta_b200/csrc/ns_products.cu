@@ -14,11 +14,11 @@
 // All sides are padded to 128 with zeros that reproduce themselves, so nothing is masked here except
 // the second half of a 256-row or 256-column tile at the edge.
 //
-// One persistent, cooperative launch runs all stages of all matrices: the tile list holds stage after
-// stage, every CTA (pair) walks its share in order, and a tile starts once all tiles of the same
-// matrix's earlier stages are stored (a counter per matrix; release by the storing warps, acquire by the
-// loading ones).  A tile waits only for tiles before it in the list and all CTAs are resident, so the first
-// unfinished tile can always run.  Against one launch per stage this saves the launches' fill and drain
+// One persistent, cooperative launch runs all stages of all matrices: every CTA (pair) walks a list of tiles
+// that the planner made for it, and a tile starts once all tiles of the same matrix's earlier stages are
+// stored (a counter per matrix; release by the storing warps, acquire by the loading ones).  The lists follow
+// one order of all tiles in which a tile comes after those it waits for, and all CTAs are resident, so the
+// first unfinished tile can always run.  Against one launch per stage this saves the launches' fill and drain
 // (10 us a stage for a 256 x 784 matrix by itself) and lets other matrices' tiles fill the gaps between the
 // stages of one.
 //
@@ -127,7 +127,7 @@ struct Tile {
     uint32_t after;
     bool mirror, shared, b_mn, skipped;
 };
-__device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *active, int t)
+__device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *active, int t, int end)
 {
     Tile ti;
     ti.p = l.problems;
@@ -136,7 +136,7 @@ __device__ __forceinline__ Tile fetch_tile(const NsLaunch &l, const uint32_t *ac
     ti.after = 0;
     ti.mirror = ti.shared = ti.b_mn = false;
     ti.skipped = true;
-    if (t < l.n_tiles) {
+    if (t < end) {
         const NsTile tile = l.tiles[t];
         const NsProduct *p = l.problems + tile.problem;
         ti.p = p;
@@ -359,9 +359,8 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     const int warp = uniform((int)(threadIdx.x >> 5));
     const int lane = threadIdx.x & 31;
     const uint32_t cta_rank = kCtas == 2 ? cluster_ctarank() : 0u;
-    const int group_id = blockIdx.x / kCtas;
-    const int n_groups = gridDim.x / kCtas;
-    int n_tiles = launch.n_tiles;
+    const int first_tile = launch.begin[blockIdx.x / kCtas];
+    int end = launch.begin[blockIdx.x / kCtas + 1];
     constexpr uint32_t kArrivals = kCtas * kEpiWarps;  // on a matrix's counter, per tile
 
     if (threadIdx.x == 0) {
@@ -398,7 +397,7 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
     if (kCtas == 2) cluster_sync_all();
     tcgen05_fence_after();
     const uint32_t tmem_base = bars->tmem_base;
-    if (bars->skip != 0u) n_tiles = 0;  // an earlier call gave up a wait
+    if (bars->skip != 0u) end = first_tile;  // an earlier call gave up a wait
 
     if (warp == 0) {
         // ---- TMA producer ----
@@ -410,10 +409,10 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         // the leader announces the bytes of both CTAs; the peer's may land before that, the phase cannot end before it
         const uint32_t my_full0 = uniform(smem_u32(&bars->full[0]));
         const uint32_t full0 = uniform(kCtas == 2 ? map_to_cta(my_full0, 0) : my_full0);
-        Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
-        for (int t = group_id; t < n_tiles && ok; t += n_groups) {
+        Tile next = fetch_tile(launch, active, first_tile, end);
+        for (int t = first_tile; t < end && ok; ++t) {
             const Tile ti = uniform_tile(next);
-            next = fetch_tile(launch, active, t + n_groups);
+            next = fetch_tile(launch, active, t + 1, end);
             if (ti.skipped) continue;
             const int a_row0 = ti.m0 + (int)cta_rank * BM, b_row0 = ti.n0 + (int)cta_rank * C::kBRows;
             const int plane_rows = uniform(ti.p->plane_rows);
@@ -469,10 +468,10 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
             const uint64_t desc_k = operand_desc(base, false, 0), desc_mn = operand_desc(base, true, 0);
             const uint32_t full0 = uniform(smem_u32(&bars->full[0])), empty0 = uniform(smem_u32(&bars->empty[0]));
             const uint32_t tmem = uniform(tmem_base);
-            Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
-            for (int t = group_id; t < n_tiles && ok; t += n_groups) {
+            Tile next = fetch_tile(launch, active, first_tile, end);
+            for (int t = first_tile; t < end && ok; ++t) {
                 const Tile ti = uniform_tile(next);
-                next = fetch_tile(launch, active, t + n_groups);
+                next = fetch_tile(launch, active, t + 1, end);
                 if (ti.skipped) continue;
                 const uint32_t idesc = make_idesc(ti.b_mn, BM * kCtas, C::BN);
                 // B's descriptor differs by its major-ness in the fields above the address and in the step of a k slice
@@ -540,10 +539,10 @@ ns_product_kernel(const NsLaunch launch, const uint32_t *active, const NsError e
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        Tile next = fetch_tile(launch, active, n_tiles > 0 ? group_id : launch.n_tiles);
-        for (int t = group_id; t < n_tiles && ok; t += n_groups) {
+        Tile next = fetch_tile(launch, active, first_tile, end);
+        for (int t = first_tile; t < end && ok; ++t) {
             const Tile ti = next;
-            next = fetch_tile(launch, active, t + n_groups);
+            next = fetch_tile(launch, active, t + 1, end);
             if (ti.skipped) continue;
             const NsProduct *p = ti.p;
             float mult = 1.0f;
@@ -714,7 +713,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 template <int kCtas, int kPlanes>
-int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, int sm_count, cudaStream_t stream,
+int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, cudaStream_t stream,
                    uint32_t wait_limit, bool withhold)
 {
     const size_t smem = smem_bytes<kCtas, kPlanes>();
@@ -732,30 +731,38 @@ int launch_variant(const NsLaunch &l, const uint32_t *d_active, NsError error, i
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = kCtas == 2 ? 2 : 1;
-    int resident = sm_count;
-    if (kCtas == 2) {
-        static int max_clusters = 0;  // a device function of the kernel: pairs that fit at once
-        if (max_clusters == 0) {
-            cfg.gridDim = dim3((unsigned)(sm_count / 2 * 2));
-            cudaLaunchAttribute only[1] = {attr[1]};
-            cfg.attrs = only;
-            cfg.numAttrs = 1;
-            int count = 0;
-            VB_CUDA(cudaOccupancyMaxActiveClusters(&count, ns_product_kernel<kCtas, kPlanes>, &cfg));
-            if (count < 1) return fail(VB_ERR_CUDA, "the device cannot hold a 2-CTA cluster of the product kernel");
-            max_clusters = count;
-            cfg.attrs = attr;
-            cfg.numAttrs = 2;
-        }
-        resident = std::min(sm_count, 2 * max_clusters);
-    }
-    const int groups = std::min(resident / kCtas, l.widest);
-    cfg.gridDim = dim3((unsigned)(groups * kCtas));
+    cfg.gridDim = dim3((unsigned)(l.groups * kCtas));
     VB_CUDA(cudaLaunchKernelEx(&cfg, ns_product_kernel<kCtas, kPlanes>, l, d_active, error, wait_limit, withhold ? 1 : 0));
     return VB_OK;
 }
 
 }  // namespace
+
+int ns_resident_groups(int shape, int planes, int sm_count, int *groups)
+{
+    *groups = sm_count;
+    if (shape != NS_TILE_PAIR) return VB_OK;
+    // pairs are the two SMs of a TPC; where an SM of one is missing, fewer fit than half of the SMs
+    auto *kernel = planes == 2 ? ns_product_kernel<2, 2> : ns_product_kernel<2, 1>;
+    const size_t smem = planes == 2 ? smem_bytes<2, 2>() : smem_bytes<2, 1>();
+    VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3((unsigned)(sm_count / 2 * 2));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    VB_CUDA(cudaOccupancyMaxActiveClusters(&count, kernel, &cfg));
+    if (count < 1) return fail(VB_ERR_CUDA, "the device cannot hold a 2-CTA cluster of the product kernel");
+    *groups = std::min(count, sm_count / 2);
+    return VB_OK;
+}
 
 void ns_tile_extent(int shape, int planes, int *bm, int *bn)
 {
@@ -788,14 +795,14 @@ int make_ns_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer
 }
 
 int launch_ns_products(const NsLaunch &l, int shape, int planes, const uint32_t *d_active, NsError error,
-                       int sm_count, cudaStream_t stream, uint32_t wait_limit, bool withhold)
+                       cudaStream_t stream, uint32_t wait_limit, bool withhold)
 {
     if (l.n_tiles <= 0) return VB_OK;
     if (shape == NS_TILE_PAIR)
-        return planes == 2 ? launch_variant<2, 2>(l, d_active, error, sm_count, stream, wait_limit, withhold)
-                           : launch_variant<2, 1>(l, d_active, error, sm_count, stream, wait_limit, withhold);
-    return planes == 2 ? launch_variant<1, 2>(l, d_active, error, sm_count, stream, wait_limit, withhold)
-                       : launch_variant<1, 1>(l, d_active, error, sm_count, stream, wait_limit, withhold);
+        return planes == 2 ? launch_variant<2, 2>(l, d_active, error, stream, wait_limit, withhold)
+                           : launch_variant<2, 1>(l, d_active, error, stream, wait_limit, withhold);
+    return planes == 2 ? launch_variant<1, 2>(l, d_active, error, stream, wait_limit, withhold)
+                       : launch_variant<1, 1>(l, d_active, error, stream, wait_limit, withhold);
 }
 
 }  // namespace vb
