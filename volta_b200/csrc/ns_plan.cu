@@ -366,15 +366,16 @@ int gram_parts(const NsProduct &pr, int shape, uint32_t stage_tiles, int sm_coun
     return std::max(1, std::min(pr.K / kNsKBlock / 8, sm_count / (int)stage_tiles));
 }
 
-constexpr double kTileCycles[2][2] = {{11.9, 10.5}, {18.4, 18.7}};  // per element of the contraction: [planes - 1][shape]
+constexpr double kTileCycles[2][2] = {{8.0, 9.1}, {15.6, 17.0}};  // per element of the contraction: [planes - 1][shape]
 
 // The shape whose stages take less time if every stage is waited for: whole rounds of tiles over the device's
-// CTAs (pairs), at the measured cycles of a tile per element of the contraction, plus what a stage costs
-// besides (signals, first loads, epilogue: about 12000 cycles).  One plane: a 128 x 128 tile takes 10.5 cycles
-// (issue bound), a pair's 256 x 256 one 11.9 (bound by L2); two planes 18.7 and, 256 x 128, 18.4.
+// CTAs (pairs), at the measured cycles of a tile per element of the contraction (one plane: 128 x 128 9.1, issue bound,
+// 256 x 256 by a pair 8.0, the tensor core's rate; two planes 17.0 and, 256 x 128, 15.6), plus what a stage costs
+// besides: signals, first loads and epilogue, 12000 cycles, 19000 with the pair's 256 columns (1000 x 513 bf16: 125 us with
+// 128 x 128 tiles, 180 with the pair's).
 int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t> &stage_begin, int planes, int sm_count)
 {
-    const double per_stage = 12000.0;
+    const double per_stage[2] = {planes == 1 ? 19000.0 : 12000.0, 12000.0};
     double cost[2] = {0.0, 0.0};
     for (int shape = 0; shape < 2; ++shape) {
         const double groups = shape == NS_TILE_PAIR ? sm_count / 2 : sm_count;
@@ -391,7 +392,7 @@ int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t>
             }
             if (tiles == 0) continue;
             const double rounds = std::ceil(tiles / groups), mean = work / tiles;
-            cost[shape] += per_stage * (cut ? 2 : 1) + kTileCycles[planes - 1][shape] * std::max(longest, cut ? work / groups : rounds * mean);
+            cost[shape] += per_stage[shape] * (cut ? 2 : 1) + kTileCycles[planes - 1][shape] * std::max(longest, cut ? work / groups : rounds * mean);
         }
     }
     return cost[NS_TILE_PAIR] <= cost[NS_TILE_128] ? NS_TILE_PAIR : NS_TILE_128;
@@ -400,7 +401,7 @@ int pick_shape(const std::vector<NsProduct> &problems, const std::vector<size_t>
 // Deals the tiles out to the groups: the device is played through with the measured cost of a tile (see pick_shape), a
 // free group takes a tile of the matrix that has the longest way to go among those whose last stage is stored by
 // then.  So a long contraction of one matrix does not hold up the stages of the others, as it does where tiles are dealt
-// round robin (one d = 1024 transformer layer: 320 us).  A stage is dealt after the one before it: every group's
+// round robin (bf16 products of 2 x (300x2000), 3 x (700x700), 10 x (200x200): 179 against 166 us).  A stage is dealt after the one before it: every group's
 // list follows the order of dealing, in which a tile comes after those it waits for.
 void deal_tiles(const std::vector<NsTile> &tiles, const std::vector<NsProduct> &problems, int64_t n_matrices, double cycles_per_k,
                 int groups, std::vector<NsTile> *dealt, std::vector<int32_t> *begin)
