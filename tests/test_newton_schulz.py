@@ -277,8 +277,9 @@ def test_orthogonalize_in_place_zero_tiny_huge_and_undefined(engine, shape, mode
 
 @gpu
 @pytest.mark.parametrize("mode", ["f16", "f32"])
-@pytest.mark.parametrize("coefficients", [QUINTIC[:1], [(2.0, -1.5, 0.5)] * 12, [(1.0, 0.0, 0.0)] * 2, [(1.5, -0.5, 0.0)] * 20],
-                         ids=["one", "twelve", "identity", "twenty linear"])
+@pytest.mark.parametrize("coefficients", [QUINTIC[:1], [(2.0, -1.5, 0.5)] * 12, [(1.0, 0.0, 0.0)] * 2, [(1.5, -0.5, 0.0)] * 20,
+                                          [(1.0, 0.0, 1e-20)] * 40, [(1.9, 0.0, 0.0)] * 6],
+                         ids=["one", "twelve", "identity", "twenty linear", "more than a small program holds", "growing"])
 def test_other_step_counts(engine, coefficients, mode):
     import torch
     import volta_b200 as vb

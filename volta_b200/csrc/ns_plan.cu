@@ -472,7 +472,6 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
     std::vector<Schedule> schedules;       // the different ones among the matrices
     std::vector<std::vector<std::vector<int>>> groupings;
     std::map<std::pair<double, double>, size_t> by_limits;
-    std::vector<std::vector<NsSmallOp>> programs;
     std::vector<size_t> kind((size_t)n);
     std::vector<NsSmallMatrix> small;
     std::vector<NsSmallOp> small_ops;
@@ -566,7 +565,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
 
     // The carving is done twice: for the size, then with the addresses (tensor maps need them).
     __half *x_base = nullptr, *square_base = nullptr;
-    for (int round = 0; round < 2; ++round) {
+    for (int pass = 0; pass < 2; ++pass) {
         Carver c;
         c.base = p->d_base;
         x_base = c.take<__half>((size_t)(2 * x_total));
@@ -615,7 +614,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
                     q.matrix = (int32_t)i;
                     q.flags = (pr.update ? NS_B_MN_MAJOR : 0) | (pr.gram ? NS_GRAM : 0) |
                               (pr.A == pr.B && !pr.update ? NS_SAME : 0);
-                    if (round == 1) {
+                    if (pass == 1) {
                         const int64_t outer = (int64_t)p->planes * d.np;
                         VB_TRY(make_ns_map(&q.map_a, address(pr.A), q.K, outer, NS_MAP_ROWS));
                         const bool narrow = p->planes == 2 && p->shape == NS_TILE_PAIR;  // 64 rows of B per CTA
@@ -697,14 +696,14 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
         int32_t *d_begin = c.take<int32_t>((size_t)groups + 1);
         p->products = {d_problems, d_tiles, d_begin, p->ew.stored, partials, (int)tile_list.size(), groups};
         std::vector<int32_t> begin;
-        if (round == 1) {
+        if (pass == 1) {
             std::vector<NsTile> dealt;
             deal_tiles(tile_list, problems, n, kTileCycles[p->planes - 1][p->shape], groups, &dealt, &begin);
             tile_list.swap(dealt);
             VB_CUDA(cudaMemcpyAsync(d_begin, begin.data(), begin.size() * sizeof(int32_t), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaStreamSynchronize(p->eng->stream));  // `begin` goes out of scope
         }
-        if (round == 1) {
+        if (pass == 1) {
             VB_CUDA(cudaMemcpyAsync(d_problems, problems.data(), problems.size() * sizeof(NsProduct), cudaMemcpyHostToDevice, p->eng->stream));
             VB_CUDA(cudaMemcpyAsync(d_tiles, tile_list.data(), tile_list.size() * sizeof(NsTile), cudaMemcpyHostToDevice, p->eng->stream));
             int bm, bn;
@@ -718,7 +717,7 @@ int build_plan(vb_ns_plan *p, const std::vector<Step> &steps)
             for (const NsTile &t : tile_list)
                 p->flops += 2.0 * (p->planes == 2 ? 3.0 : 1.0) * bm * bn * (double)(t.kb1 - t.kb0) * kNsKBlock;
         }
-        if (round == 0) {
+        if (pass == 0) {
             p->workspace = c.used;
             const cudaError_t err = cudaMalloc((void **)&p->d_base, std::max<size_t>(c.used, 1024));
             if (err != cudaSuccess) {
