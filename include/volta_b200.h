@@ -528,7 +528,8 @@ int vb_multi_tensor_step_static(vb_engine *engine, const vb_optimizer_step_param
  * ns_mode: VB_NS_F16 holds every iterate in f16 (times a power of two; the error of O is about
  * 1e-3 relative on gradients with a floor of noise; singular directions that the input holds
  * below about 2^-11 / sqrt(n) of the largest are lost, as in any 16-bit arithmetic), VB_NS_F32_TC in two f16
- * planes (about 1e-6).  The other modes return VB_ERR_UNSUPPORTED.
+ * planes (1e-6 to 1e-5, most where steep coefficients meet a
+ * short side of 17 to 30).  The other modes return VB_ERR_UNSUPPORTED.
  *
  * A matrix may have a side of 1 or 0; sides up to 65536.  A U of zeros gives zeros (eps > 0); a U
  * with an infinity or a NaN gives NaN for that matrix and leaves the others as they are.  Results do not depend on

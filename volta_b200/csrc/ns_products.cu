@@ -24,9 +24,9 @@
 //
 // Warp roles as in ns_gemm_tc.cu: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue with two
 // accumulators.  Two shapes:
-//   256 x 256 (two planes: 256 x 128) by a CTA pair (cta_group::2): half the operand traffic per FLOP.  With one plane
-//             that traffic (L2 to shared memory) is what bounds large products: with B not loaded at all they ran
-//             at 1350 instead of 1072 TFLOP/s.  Two planes do three products on what they load; there 256 columns
+//   256 x 256 (two planes: 256 x 128) by a CTA pair (cta_group::2): half the operand traffic per FLOP; the mainloop runs
+//             at the tensor core's rate (512 cycles per 64 of the contraction), large products at 1.0 to 1.15 PFLOP/s under
+//             the power cap (1.45 to 1.55 GHz).  Two planes do three products on what they load; there 256 columns
 //             only cost registers (the sums spilled) and parallelism (2048 x 2048 f32: 870 us against 785)
 //   128 x 128 by one CTA: four times as many tiles, for lists that would leave SMs idle
 // (the planner picks, see pick_shape).
