@@ -538,6 +538,48 @@ def test_captured_calls_replay(engine):
 
 
 @gpu
+@pytest.mark.parametrize("others", [[], [(200, 300)]], ids=["small only", "beside a larger one"])
+def test_launches_side_by_side_are_ordered_with_the_engine(engine, others):
+    """300 small matrices are several launches that run beside each other: the call sees what the stream wrote before
+    it and is complete for what the stream does next, at once and as a replayed graph."""
+    import torch
+    import volta_b200 as vb
+    shapes = [(96, 40)] * 300 + others
+    plan = vb.NewtonSchulzPlan(shapes, QUINTIC, engine=engine)
+    x, mid, out = ([torch.zeros(s, device="cuda") for s in shapes] for _ in range(3))
+    tx, tm, to = (plan.matrices(a) for a in (x, mid, out))
+    want = []
+    stream = torch.cuda.ExternalStream(engine.stream)
+    source = [[_gradient(torch, s, 1000 * k + i, torch.float32) for i, s in enumerate(shapes)] for k in range(3)]
+    for fresh in source:  # one call at a time
+        torch._foreach_copy_(x, fresh)
+        torch.cuda.synchronize()
+        plan.orthogonalize(tx, tm)
+        engine.synchronize()
+        plan.orthogonalize(tm, to)
+        engine.synchronize()
+        want.append([o.clone() for o in out])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        plan.orthogonalize(tx, tm)
+        plan.orthogonalize(tm, to)
+    got = []
+    with torch.cuda.stream(stream):
+        for k, fresh in enumerate(source + source):  # nothing waits on the host in between
+            torch._foreach_copy_(x, fresh)
+            if k < len(source):
+                plan.orthogonalize(tx, tm)
+                plan.orthogonalize(tm, to)
+            else:
+                graph.replay()
+            got.append([o.clone() for o in out])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, want + want) for a, b in zip(g, w))
+    plan.close()
+
+
+@gpu
 def test_refusals(engine):
     import torch
     import volta_b200 as vb

@@ -16,7 +16,7 @@
 //
 // What a stage of short-side products costs (cycles, 64 x 288 to f32 accuracy): issuing 12 MMAs 1000, their completion 300
 // to 500, tensor memory to shared memory 900, barriers 200; a Gram over a cluster of 8 takes 6500, 4300 of them the sum.
-// The whole call takes 39 us with a 32 x 9 matrix beside it; 192 bf16 heads of 1024 x 64 take 111 us, two rounds of one
+// The whole call takes 39 us with a 32 x 9 matrix beside it; 192 bf16 heads of 1024 x 64 take 107 us, two rounds of one
 // head per SM.
 //
 // A short side of at most 16 to f32 accuracy (tiny) is worked on in f64 on the CUDA cores instead: planes of 22
