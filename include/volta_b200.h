@@ -571,8 +571,8 @@ int vb_ns_matrices_create(vb_ns_plan *plan, int dtype, void *const *pointers, co
 int vb_ns_matrices_destroy(vb_ns_matrices *list);
 
 /* outputs[i] = O(inputs[i]) for every matrix.  A list whose arrays are written must not hold two
- * elements at one address; an output may be its own input (the same list).  Other overlaps are
- * the caller's to avoid. */
+ * elements at one address; an output may be its own input (the same list).  An array that starts
+ * where another matrix's does is refused; other overlaps are the caller's to avoid. */
 int vb_orthogonalize(vb_ns_plan *plan, const vb_ns_matrices *inputs, const vb_ns_matrices *outputs);
 
 /* Muon's step on the caller's buffers:

@@ -636,6 +636,80 @@ def test_refusals(engine):
 
 
 @gpu
+def test_arrays_of_another_matrix_are_refused(engine):
+    """Matrices of one call run at the same time, so none may write what another reads."""
+    import torch
+    import volta_b200 as vb
+    plan = vb.NewtonSchulzPlan([(8, 16), (8, 16)], QUINTIC, engine=engine)
+    a, b, c, d, e, f = (torch.ones(8, 16, device="cuda:0") for _ in range(6))
+    torch.cuda.synchronize()
+    for x, o in (([a, b], [b, a]), ([a, a], [a, b]), ([a, b], [c, a]), ([a, b], [b.t().t(), c])):
+        with pytest.raises(vb.VoltaB200Error, match="one address"):
+            plan.orthogonalize(x, o)
+    for p, g, v in (([a, b], [c, a], [d, e]), ([a, b], [c, d], [e, c]), ([a, b], [c, d], [b, e]), ([a, b], [None, a], [d, e])):
+        with pytest.raises(vb.VoltaB200Error, match="one address"):
+            plan.muon_step(p, g, v, lr=0.1)
+    plan.orthogonalize([a, a], [c, d])  # one input read twice
+    plan.orthogonalize([a, b], [a, c])  # in place
+    plan.muon_step([a, b], [c, c], [e, f], lr=0.1)
+    engine.synchronize()
+    assert torch.equal(e, f)
+
+
+@gpu
+def test_a_list_does_not_outlive_its_plan(engine):
+    """A plan that takes the place of a closed one does not accept the closed one's lists."""
+    import torch
+    import volta_b200 as vb
+    x, y = torch.ones(8, 16, device="cuda:0"), torch.ones(8, 16, device="cuda:0")
+    torch.cuda.synchronize()
+    addresses, lists, back = set(), [], False
+    for _ in range(100):
+        plan = vb.NewtonSchulzPlan([(8, 16)], QUINTIC, engine=engine)
+        back = back or plan._h.value in addresses
+        addresses.add(plan._h.value)
+        for old in lists:
+            with pytest.raises(vb.VoltaB200Error, match="another plan"):
+                plan.orthogonalize(old, [y])
+        lists.append(plan.matrices([x]))
+        plan.orthogonalize(lists[-1], [y])
+        plan.close()
+        if back:  # an allocator may also never give an address twice
+            break
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["f16", "f32"])
+@pytest.mark.parametrize("columns", [1, 3, 8, 20])
+@pytest.mark.parametrize("rows", [1, 5, 77, 300])
+def test_leading_columns_of_a_wider_array(engine, rows, columns, mode):
+    """x[:, :k] of a contiguous array whose rows are 16-byte aligned: what lies behind the k columns stays."""
+    import torch
+    import volta_b200 as vb
+    ns_mode, dtype = (vb.VB_NS_F32_TC, torch.float32) if mode == "f32" else (vb.VB_NS_F16, torch.bfloat16)
+    shape = (rows, columns)
+    plan = vb.NewtonSchulzPlan([shape, shape, shape[::-1]], QUINTIC, ns_mode=ns_mode, engine=engine)
+    wide = [torch.full((rows, 24 if columns > 8 else 8), 7.0, dtype=dtype, device="cuda:0") for _ in range(6)]
+    x, o = ([w[:, :columns] for w in ws] for ws in (wide[:3], wide[3:]))
+    for i, m in enumerate(x):
+        m.copy_(_gradient(torch, shape, 40 + i, dtype))
+    x[2], o[2] = x[2].t(), o[2].t()
+    before = [w.clone() for w in wide]
+    torch.cuda.synchronize()
+    plan.orthogonalize(x, o)
+    engine.synchronize()
+    for a, b in zip(x, o):
+        want, bound = _exact(a.double(), QUINTIC)
+        _close(b, want, bound, _unit(ns_mode, a.shape), dtype)
+    v = [torch.zeros_like(m) for m in x]
+    plan.muon_step(o, x, v, lr=0.1)
+    engine.synchronize()
+    for w, b in zip(wide, before):
+        assert torch.equal(w[:, columns:], b[:, columns:])
+    assert all(torch.equal(w, b) for w, b in zip(wide[:3], before[:3]))
+
+
+@gpu
 def test_producers_and_consumers_on_other_streams(engine):
     """Inputs made on one stream, outputs read on another, ordered by events against the engine's stream."""
     import torch

@@ -24,6 +24,7 @@
 #include <cmath>
 
 #include <algorithm>
+#include <atomic>
 #include <map>
 #include <functional>
 #include <memory>
@@ -264,10 +265,11 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 }  // namespace vb
 
 struct vb_ns_matrices {
-    vb_ns_plan *plan = nullptr;
+    uint64_t plan = 0;  // serial number of its plan: an address may come back after the plan is gone
     int dtype = 0;
     std::vector<vb::NsArray> arrays;  // in the working orientation
     std::vector<uint8_t> vec;         // rows (or columns) on 16-byte boundaries
+    std::vector<std::pair<const void *, int64_t>> starts;  // first addresses in order, with their matrices
     bool writable = true;             // no two elements at one address
     bool turned = false;              // an array is contiguous along the short side
     bool any_null = false;            // a matrix with elements has no array
@@ -276,6 +278,7 @@ struct vb_ns_matrices {
 
 struct vb_ns_plan {
     vb_engine *eng = nullptr;
+    uint64_t serial = 0;
     int device = 0;
     int64_t n = 0;
     std::vector<int64_t> rows, cols;
@@ -829,19 +832,26 @@ int run_plan(vb_ns_plan *p, const NsElementwise &w, bool step, bool turned, Fill
 int check_list(const vb_ns_plan *p, const vb_ns_matrices *l, const char *name, bool written, bool may_be_absent)
 {
     if (!l) return fail(VB_ERR_INVALID_ARG, "%s is null", name);
-    if (l->plan != p) return fail(VB_ERR_INVALID_ARG, "%s belongs to another plan", name);
+    if (l->plan != p->serial) return fail(VB_ERR_INVALID_ARG, "%s belongs to another plan", name);
     if (l->any_null && !may_be_absent) return fail(VB_ERR_INVALID_ARG, "%s has a null pointer", name);
     if (written && !l->writable) return fail(VB_ERR_INVALID_ARG, "%s cannot be written: %s", name, l->why);
     return VB_OK;
 }
-// Two lists may share a matrix's memory only as the very same array.
+// Two lists, of which at least one is written, may share a matrix's memory only as the very same array of the same
+// matrix.  Found by the first addresses; strided arrays may interleave otherwise.
 int check_alias(const vb_ns_matrices *a, const vb_ns_matrices *b, const char *names, bool same_allowed)
 {
-    for (size_t i = 0; i < a->arrays.size(); ++i) {
-        const NsArray &x = a->arrays[i], &y = b->arrays[i];
-        if (x.ptr == nullptr || x.ptr != y.ptr) continue;
-        if (!same_allowed || a->dtype != b->dtype || x.si != y.si || x.sj != y.sj)
-            return fail(VB_ERR_INVALID_ARG, "%s of matrix %lld start at one address", names, (long long)i);
+    size_t k = 0;
+    for (const auto &s : a->starts) {
+        while (k < b->starts.size() && std::less<const void *>()(b->starts[k].first, s.first)) ++k;
+        for (size_t q = k; q < b->starts.size() && b->starts[q].first == s.first; ++q) {
+            const NsArray &x = a->arrays[(size_t)s.second], &y = b->arrays[(size_t)b->starts[q].second];
+            if (s.second != b->starts[q].second)
+                return fail(VB_ERR_INVALID_ARG, "%s of matrices %lld and %lld start at one address", names, (long long)s.second,
+                            (long long)b->starts[q].second);
+            if (!same_allowed || a->dtype != b->dtype || x.si != y.si || x.sj != y.sj)
+                return fail(VB_ERR_INVALID_ARG, "%s of matrix %lld start at one address", names, (long long)s.second);
+        }
     }
     return VB_OK;
 }
@@ -915,6 +925,8 @@ int vb_ns_plan_create(vb_engine *e, int64_t n, const int64_t *rows, const int64_
     DeviceGuard guard;
     VB_TRY(guard.enter(e->device));
     vb_ns_plan *p = new vb_ns_plan();
+    static std::atomic<uint64_t> serials{0};
+    p->serial = ++serials;
     p->eng = e;
     p->device = e->device;
     p->n = n;
@@ -982,11 +994,11 @@ int vb_ns_matrices_create(vb_ns_plan *p, int dtype, void *const *pointers, const
     if (p->n > 0 && !pointers) return fail(VB_ERR_INVALID_ARG, "pointers is null");
     const int64_t size = dtype == VB_DTYPE_F32 ? 4 : 2, per16 = 16 / size;
     std::unique_ptr<vb_ns_matrices> l(new vb_ns_matrices());
-    l->plan = p;
+    l->plan = p->serial;
     l->dtype = dtype;
     l->arrays.resize((size_t)p->n);
     l->vec.assign((size_t)p->n, 0);
-    std::vector<const void *> seen;
+    auto &starts = l->starts;
     for (int64_t i = 0; i < p->n; ++i) {
         const int64_t rows = p->rows[i], cols = p->cols[i];
         if (rows == 0 || cols == 0) continue;
@@ -1023,10 +1035,11 @@ int vb_ns_matrices_create(vb_ns_plan *p, int dtype, void *const *pointers, const
         const bool apart = (a.sj >= 1 && a.si >= (m - 1) * a.sj + 1) || (a.si >= 1 && a.sj >= (n - 1) * a.si + 1) ||
                            (n == 1 && (a.sj >= 1 || m == 1));
         if (!apart) l->writable = false, l->why = "elements of a matrix share an address";
-        seen.push_back(a.ptr);
+        starts.emplace_back(a.ptr, i);
     }
-    std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) l->writable = false, l->why = "two matrices start at one address";
+    std::sort(starts.begin(), starts.end());
+    const auto same = [](const auto &x, const auto &y) { return x.first == y.first; };
+    if (std::adjacent_find(starts.begin(), starts.end(), same) != starts.end()) l->writable = false, l->why = "two matrices start at one address";
     *out = l.release();
     return VB_OK;
     VB_NS_END
